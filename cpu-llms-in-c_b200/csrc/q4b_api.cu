@@ -2,8 +2,10 @@
 // loader, matmul dispatch, completion/timing and graph replay.  Host code only;
 // the kernels live in q4b_pack.cu, q4b_decode.cu and q4b_gemm.cu.
 #include "../../include/q4b200.h"
+#include "q4b_cache.cuh"
 #include "q4b_kernels.h"
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -35,6 +37,8 @@ struct q4b_context {
     float *tc_workspace;      // partial tiles of the tensor-core GEMM when it splits tiles over CTAs
     size_t tc_workspace_bytes;
     uint32_t *tc_flags;
+    float *attention_partials;     // sums of query rows whose keys are split over thread blocks
+    uint32_t *attention_arrivals;  // their counters, zero between launches
 };
 
 struct q4b_weight {
@@ -550,6 +554,8 @@ void q4b_context_close(q4b_context *context) {
     cudaFree(context->tc_workspace);
     cudaFree(context->tc_flags);
     cudaFree(context->x16);
+    cudaFree(context->attention_partials);
+    cudaFree(context->attention_arrivals);
     delete context;
 }
 
@@ -957,6 +963,235 @@ int q4b_rmsnorm(q4b_context *context, const void *input, int input_dtype, const 
                                         context->stream);
     if (!context->capturing) ++context->launches;
     if (status != cudaSuccess) return device_failure(error_message, error_capacity, "rms norm", status);
+    return Q4B_OK;
+}
+
+/* ----------------------------------------------- paged cache, attention, sampling */
+namespace {
+
+int check_cache(const q4b_kv_cache *cache, const q4b_token_batch *batch, uint32_t q_heads, CacheView *cache_view,
+                BatchView *batch_view, char *error_message, size_t error_capacity) {
+    if (cache == nullptr || batch == nullptr || cache->keys == nullptr || cache->values == nullptr ||
+        !aligned16(cache->keys) || !aligned16(cache->values)) {
+        set_error(error_message, error_capacity, "no cache or batch, or its pools are missing or not 16-byte aligned");
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (cache->dtype != Q4B_F16 && cache->dtype != Q4B_BF16) {
+        set_error(error_message, error_capacity, "the cache must be fp16 or bf16");
+        return Q4B_BAD_ARGUMENT;
+    }
+    const uint32_t tokens = cache->page_tokens, head = cache->head_size;
+    if (tokens < 16 || tokens > 1024 || (tokens & (tokens - 1)) != 0 || (head != 64 && head != 128 && head != 256)) {
+        set_error(error_message, error_capacity,
+                  "page_tokens=%u must be a power of two from 16 to 1024, head_size=%u 64, 128 or 256", tokens, head);
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (cache->pages == 0 || cache->kv_heads == 0 || q_heads == 0 || q_heads % cache->kv_heads != 0) {
+        set_error(error_message, error_capacity, "pages=%u, kv_heads=%u: q_heads=%u must be a multiple of kv_heads",
+                  cache->pages, cache->kv_heads, q_heads);
+        return Q4B_BAD_ARGUMENT;
+    }
+    auto words = [](const void *pointer) { return pointer != nullptr && (reinterpret_cast<uintptr_t>(pointer) & 3u) == 0; };
+    if (batch->tokens != 0 && batch->sequences != 0 &&
+        (!words(batch->token_begin) || !words(batch->lengths) || !words(batch->page_table) || batch->table_stride == 0)) {
+        set_error(error_message, error_capacity, "token_begin, lengths or page_table missing or misaligned, or table_stride is 0");
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (batch->sequences > 0x7fffffffu || batch->tokens > 0x7fffffffu / (q_heads / cache->kv_heads)) {
+        set_error(error_message, error_capacity, "%u sequences with %u rows of %u query heads per key head are too many",
+                  batch->sequences, batch->tokens, q_heads / cache->kv_heads);
+        return Q4B_BAD_ARGUMENT;
+    }
+    *cache_view = {cache->keys, cache->values, cache->pages, tokens, 0, cache->kv_heads, head, cache->dtype};
+    while ((1u << cache_view->page_shift) < tokens) ++cache_view->page_shift;
+    *batch_view = {batch->token_begin, batch->lengths, batch->page_table, batch->sequences, batch->tokens, batch->table_stride};
+    return Q4B_OK;
+}
+
+// [rows][stride] with `width` values used of every row: does [a, ...) touch [b, ...)?
+struct Block {
+    const void *pointer;
+    uint32_t rows;
+    uint64_t stride_bytes, width_bytes;
+    uintptr_t begin() const { return reinterpret_cast<uintptr_t>(pointer); }
+    uintptr_t end() const { return begin() + (uintptr_t)((uint64_t)(rows - 1) * stride_bytes + width_bytes); }
+};
+bool overlap(const Block &a, const Block &b) { return a.begin() < b.end() && b.begin() < a.end(); }
+
+}  // namespace
+
+int q4b_rope_append(q4b_context *context, const q4b_kv_cache *cache, const q4b_token_batch *batch, const q4b_rope *rope,
+                    const void *q, uint32_t ldq, uint32_t q_head_stride, const void *k, uint32_t ldk, const void *v,
+                    uint32_t ldv, int dtype, uint32_t q_heads, void *q_out, uint32_t ldq_out,
+                    char *error_message, size_t error_capacity) {
+    int code = check_context(context, error_message, error_capacity);
+    if (code != Q4B_OK) return code;
+    AppendArgs args = {};
+    code = check_cache(cache, batch, q_heads, &args.cache, &args.batch, error_message, error_capacity);
+    if (code != Q4B_OK) return code;
+    const uint32_t head = cache->head_size;
+    if (rope == nullptr || rope->rotary_size > head || rope->rotary_size % 16 != 0 ||
+        (rope->pairing != Q4B_ROPE_HALVES && rope->pairing != Q4B_ROPE_NEIGHBOURS) ||
+        (rope->frequencies == nullptr && rope->rotary_size != 0 && !(rope->base > 0.0 && std::isfinite(rope->base)))) {
+        set_error(error_message, error_capacity,
+                  "no rotation, or rotary_size is no multiple of 16 up to %u, or pairing or base is invalid", head);
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (dtype != Q4B_F16 && dtype != Q4B_F32 && dtype != Q4B_BF16) {
+        set_error(error_message, error_capacity, "q, k and v must be fp16, fp32 or bf16");
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (batch->tokens == 0 || batch->sequences == 0) return Q4B_OK;
+    const size_t item = dtype_bytes(dtype);
+    const uint64_t q_width = (uint64_t)(q_heads - 1) * q_head_stride + head, kv_width = (uint64_t)cache->kv_heads * head;
+    if (q == nullptr || k == nullptr || v == nullptr || q_out == nullptr || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
+        !aligned16(q_out) || (rope->positions != nullptr && (reinterpret_cast<uintptr_t>(rope->positions) & 3u) != 0)) {
+        set_error(error_message, error_capacity, "q, k, v or q_out missing or not 16-byte aligned");
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (q_head_stride < head || ldq < q_width || ldk < kv_width || ldv < kv_width || ldq_out < (uint64_t)q_heads * head ||
+        ldq * item % 16 != 0 || q_head_stride * item % 16 != 0 || ldk * item % 16 != 0 || ldv * item % 16 != 0 ||
+        ldq_out % 8 != 0) {
+        set_error(error_message, error_capacity,
+                  "a stride is shorter than its row or no multiple of 16 bytes: ldq=%u q_head_stride=%u ldk=%u ldv=%u ldq_out=%u",
+                  ldq, q_head_stride, ldk, ldv, ldq_out);
+        return Q4B_BAD_ARGUMENT;
+    }
+    const Block out_block = {q_out, batch->tokens, (uint64_t)ldq_out * 2, (uint64_t)q_heads * head * 2};
+    const bool in_place = q == q_out && dtype == cache->dtype && q_head_stride == head && ldq == ldq_out;
+    if (!in_place && (overlap(out_block, {q, batch->tokens, ldq * item, q_width * item}) ||
+                      overlap(out_block, {k, batch->tokens, ldk * item, kv_width * item}) ||
+                      overlap(out_block, {v, batch->tokens, ldv * item, kv_width * item}))) {
+        set_error(error_message, error_capacity, "q_out overlaps q, k or v (only q itself with the same type and strides may be)");
+        return Q4B_BAD_ARGUMENT;
+    }
+    args.q = q;
+    args.k = k;
+    args.v = v;
+    args.q_out = q_out;
+    args.positions = rope->positions;
+    args.ldq = ldq;
+    args.q_head_stride = q_head_stride;
+    args.ldk = ldk;
+    args.ldv = ldv;
+    args.ldq_out = ldq_out;
+    args.q_heads = q_heads;
+    args.rotary_size = rope->rotary_size;
+    args.pairing = rope->pairing;
+    args.dtype = dtype;
+    for (uint32_t i = 0; i < rope->rotary_size / 2; ++i) {
+        const double frequency = rope->frequencies != nullptr ? rope->frequencies[i]
+                                                              : std::pow(rope->base, -2.0 * i / rope->rotary_size);
+        if (!std::isfinite(frequency)) {
+            set_error(error_message, error_capacity, "frequency %u is not finite", i);
+            return Q4B_BAD_ARGUMENT;
+        }
+        args.turns[i] = frequency / 6.283185307179586476925;
+    }
+    args.status = context->status_device;
+    cudaError_t status = launch_append(args, context->stream);
+    if (!context->capturing) ++context->launches;
+    if (status != cudaSuccess) return device_failure(error_message, error_capacity, "rope append launch", status);
+    return Q4B_OK;
+}
+
+int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_token_batch *batch, const void *q,
+                  uint32_t ldq, uint32_t q_heads, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
+                  char *error_message, size_t error_capacity) {
+    int code = check_context(context, error_message, error_capacity);
+    if (code != Q4B_OK) return code;
+    AttentionArgs args = {};
+    code = check_cache(cache, batch, q_heads, &args.cache, &args.batch, error_message, error_capacity);
+    if (code != Q4B_OK) return code;
+    if (!std::isfinite(scale)) {
+        set_error(error_message, error_capacity, "scale is not finite");
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (batch->tokens == 0 || batch->sequences == 0) return Q4B_OK;
+    const uint64_t width = (uint64_t)q_heads * cache->head_size;
+    if (q == nullptr || out == nullptr || !aligned16(q) || !aligned16(out)) {
+        set_error(error_message, error_capacity, "q or out missing or not 16-byte aligned");
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (ldq < width || ldo < width || ldq % 8 != 0 || ldo % 8 != 0) {
+        set_error(error_message, error_capacity, "ldq=%u and ldo=%u must be multiples of 8 and hold %llu values", ldq, ldo,
+                  (unsigned long long)width);
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (overlap({q, batch->tokens, (uint64_t)ldq * 2, width * 2}, {out, batch->tokens, (uint64_t)ldo * 2, width * 2})) {
+        set_error(error_message, error_capacity, "out overlaps q");
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (context->attention_arrivals == nullptr) {  // once per context, the same for every call
+        if (context->capturing) {
+            set_error(error_message, error_capacity,
+                      "the first attention of a context allocates its workspace; run it once before recording");
+            return Q4B_BAD_ARGUMENT;
+        }
+        const size_t arrival_bytes = attention_arrival_bytes(context->sm_count);
+        uint32_t *arrivals = nullptr;
+        cudaError_t status = context->attention_partials != nullptr
+                                 ? cudaSuccess
+                                 : cudaMalloc(&context->attention_partials, attention_partial_bytes(context->sm_count));
+        if (status == cudaSuccess) status = cudaMalloc(&arrivals, arrival_bytes);
+        if (status == cudaSuccess) status = cudaMemsetAsync(arrivals, 0, arrival_bytes, context->stream);
+        if (status != cudaSuccess) {
+            cudaFree(arrivals);
+            return device_failure(error_message, error_capacity, "attention workspace", status);
+        }
+        context->attention_arrivals = arrivals;
+    }
+    args.q = q;
+    args.out = out;
+    args.ldq = ldq;
+    args.ldo = ldo;
+    args.q_heads = q_heads;
+    args.group = q_heads / cache->kv_heads;
+    args.most_tokens = batch->most_tokens < batch->tokens ? batch->most_tokens : batch->tokens;
+    args.scale = scale;
+    args.window = window;
+    args.sinks = sinks;
+    args.partials = context->attention_partials;
+    args.arrivals = context->attention_arrivals;
+    args.status = context->status_device;
+    cudaError_t status = launch_attention(args, context->sm_count, context->stream);
+    if (!context->capturing) ++context->launches;
+    if (status != cudaSuccess) return device_failure(error_message, error_capacity, "attention launch", status);
+    return Q4B_OK;
+}
+
+int q4b_sample(q4b_context *context, const void *logits, int dtype, uint32_t rows, uint32_t vocab, uint32_t ld,
+               const q4b_sampling *rules, const float *uniform, uint32_t *tokens, float *probabilities,
+               char *error_message, size_t error_capacity) {
+    int code = check_context(context, error_message, error_capacity);
+    if (code != Q4B_OK) return code;
+    if (dtype != Q4B_F16 && dtype != Q4B_F32 && dtype != Q4B_BF16) {
+        set_error(error_message, error_capacity, "logits must be fp32, fp16 or bf16");
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (vocab == 0 || vocab > (1u << 20) || ld < vocab || rows > (1u << 24)) {
+        set_error(error_message, error_capacity, "vocab=%u must be 1 to 2^20, ld=%u at least that, rows=%u at most 2^24", vocab,
+                  ld, rows);
+        return Q4B_BAD_ARGUMENT;
+    }
+    if (rows == 0) return Q4B_OK;
+    auto words = [](const void *pointer) { return (reinterpret_cast<uintptr_t>(pointer) & 3u) == 0; };
+    if (logits == nullptr || uniform == nullptr || tokens == nullptr || !words(uniform) || !words(tokens) ||
+        !words(probabilities) || (reinterpret_cast<uintptr_t>(logits) & (dtype_bytes(dtype) - 1)) != 0 ||
+        (rules != nullptr && (!words(rules->temperature) || !words(rules->top_k) || !words(rules->top_p) || !words(rules->min_p)))) {
+        set_error(error_message, error_capacity, "logits, uniform or tokens missing, or an array is not aligned to its type");
+        return Q4B_BAD_ARGUMENT;
+    }
+    SampleArgs args = {logits, dtype, rows, vocab, ld, nullptr, nullptr, nullptr, nullptr, uniform, tokens, probabilities};
+    if (rules != nullptr) {
+        args.temperature = rules->temperature;
+        args.top_k = rules->top_k;
+        args.top_p = rules->top_p;
+        args.min_p = rules->min_p;
+    }
+    cudaError_t status = launch_sample(args, context->stream);
+    if (!context->capturing) ++context->launches;
+    if (status != cudaSuccess) return device_failure(error_message, error_capacity, "sample launch", status);
     return Q4B_OK;
 }
 
@@ -1519,7 +1754,16 @@ int q4b_sync(q4b_context *context, double *device_ms, char *error_message, size_
     if (*context->status_host != 0) {
         const uint32_t code = *context->status_host;
         *context->status_host = 0;
+        if (code & kBadDescriptor) {
+            set_error(error_message, error_capacity, "a token batch does not hold together: %s; results of that call are invalid",
+                      code == kBadPage ? "the page table names a page that the cache does not have"
+                      : code == kBadLength ? "a sequence is longer than its page table"
+                                           : "token_begin falls or passes the rows of the call");
+            return Q4B_BAD_ARGUMENT;
+        }
         if (context->counters != nullptr) cudaMemset(context->counters, 0, context->counter_bytes);
+        if (context->attention_arrivals != nullptr)
+            cudaMemset(context->attention_arrivals, 0, attention_arrival_bytes(context->sm_count));
         set_error(error_message, error_capacity,
                   "a device-side wait expired (code 0x%x); results of the queued work are invalid", code);
         return Q4B_DEVICE_FAILURE;

@@ -130,6 +130,62 @@ cudaError_t launch_sequence(const SequenceLaunch &launch, cudaStream_t stream);
 cudaError_t decode_static_scratch(float **scratch, uint32_t **counters, size_t *scratch_bytes,
                                   size_t *counter_bytes);
 
+// ---- q4b_append.cu, q4b_attention.cu: the paged cache ----
+struct CacheView {
+    void *keys, *values;  // [pages][kv_heads][page_tokens][head_size]
+    uint32_t pages, page_tokens, page_shift, kv_heads, head_size;
+    int dtype;
+};
+struct BatchView {
+    const uint32_t *begin, *lengths, *table;
+    uint32_t sequences, tokens, table_stride;
+};
+struct AppendArgs {
+    CacheView cache;
+    BatchView batch;
+    const void *q, *k, *v;
+    void *q_out;
+    const int32_t *positions;
+    uint32_t ldq, q_head_stride, ldk, ldv, ldq_out, q_heads;
+    uint32_t rotary_size;
+    int pairing, dtype;
+    double turns[128];  // frequency(i) / 2 pi: full turns per position
+    uint32_t *status;
+};
+cudaError_t launch_append(const AppendArgs &args, cudaStream_t stream);
+
+struct AttentionArgs {
+    CacheView cache;
+    BatchView batch;
+    const void *q;
+    void *out;
+    uint32_t ldq, ldo, q_heads, group;  // group = q_heads / kv_heads
+    uint32_t most_tokens;
+    float scale;
+    uint32_t window, sinks;
+    float *partials;       // attention_workspace_bytes of scratch; its tail holds arrival counters, zero between launches
+    uint32_t *arrivals;
+    uint32_t *status;
+};
+// what every attention launch of a device may use: sums of split rows and their counters
+size_t attention_partial_bytes(int sm_count);
+size_t attention_arrival_bytes(int sm_count);
+cudaError_t launch_attention(const AttentionArgs &args, int sm_count, cudaStream_t stream);
+
+// ---- q4b_sample.cu ----
+struct SampleArgs {
+    const void *logits;
+    int dtype;
+    uint32_t rows, vocab, ld;
+    const float *temperature;
+    const uint32_t *top_k;
+    const float *top_p, *min_p;
+    const float *uniform;
+    uint32_t *tokens;
+    float *probabilities;
+};
+cudaError_t launch_sample(const SampleArgs &args, cudaStream_t stream);
+
 // ---- q4b_gemm.cu: tcgen05 prefill GEMM ----
 struct TcGemmArgs {
     WeightView w[kMaxSegments];  // matrices that share x (same K), one launch

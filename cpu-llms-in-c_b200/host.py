@@ -14,6 +14,7 @@ import re
 import numpy as np
 
 F16, F32, BF16, NONE = 0, 1, 2, -1
+ROPE_HALVES, ROPE_NEIGHBOURS = 0, 1
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _HEADER = os.path.join(os.path.dirname(_HERE), "include", "q4b200.h")
 _ERR = 512
@@ -36,6 +37,36 @@ def declared_symbols() -> list[str]:
         text = handle.read()
     text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
     return sorted(set(re.findall(r"\b(q4b_[a-z0-9_]+)\s*\(", text)))
+
+
+class KVCache(ctypes.Structure):
+    """One layer's paged cache (q4b_kv_cache): device pointers of [pages, kv_heads, page_tokens, head_size] pools."""
+
+    _fields_ = [("keys", ctypes.c_void_p), ("values", ctypes.c_void_p), ("dtype", ctypes.c_int),
+                ("pages", ctypes.c_uint32), ("page_tokens", ctypes.c_uint32), ("kv_heads", ctypes.c_uint32),
+                ("head_size", ctypes.c_uint32)]
+
+
+class TokenBatch(ctypes.Structure):
+    """The new tokens of one call (q4b_token_batch): token_begin, lengths and page_table are device pointers."""
+
+    _fields_ = [("sequences", ctypes.c_uint32), ("tokens", ctypes.c_uint32), ("most_tokens", ctypes.c_uint32),
+                ("token_begin", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("page_table", ctypes.c_void_p),
+                ("table_stride", ctypes.c_uint32)]
+
+
+class Rope(ctypes.Structure):
+    """The rotation (q4b_rope): frequencies is a host array of doubles, positions a device pointer, both optional."""
+
+    _fields_ = [("rotary_size", ctypes.c_uint32), ("pairing", ctypes.c_int), ("base", ctypes.c_double),
+                ("frequencies", ctypes.POINTER(ctypes.c_double)), ("positions", ctypes.c_void_p)]
+
+
+class Sampling(ctypes.Structure):
+    """The rules of q4b_sample: device pointers, None is off."""
+
+    _fields_ = [("temperature", ctypes.c_void_p), ("top_k", ctypes.c_void_p), ("top_p", ctypes.c_void_p),
+                ("min_p", ctypes.c_void_p)]
 
 
 _lib = None
@@ -102,6 +133,11 @@ def library() -> ctypes.CDLL:
         "q4b_barrier_free": (None, [_vp, _vp]),
         "q4b_embedding_lookup": (_int, [_vp, _vp, _vp, _u32, _vp, _int] + err),
         "q4b_rmsnorm": (_int, [_vp, _vp, _int, _vp, _vp, _u32, _u32, ctypes.c_float] + err),
+        "q4b_rope_append": (_int, [_vp, ctypes.POINTER(KVCache), ctypes.POINTER(TokenBatch), ctypes.POINTER(Rope), _vp,
+                                   _u32, _u32, _vp, _u32, _vp, _u32, _int, _u32, _vp, _u32] + err),
+        "q4b_attention": (_int, [_vp, ctypes.POINTER(KVCache), ctypes.POINTER(TokenBatch), _vp, _u32, _u32,
+                                 ctypes.c_float, _u32, _u32, _vp, _u32] + err),
+        "q4b_sample": (_int, [_vp, _vp, _int, _u32, _u32, _u32, ctypes.POINTER(Sampling), _vp, _vp, _vp] + err),
         "q4b_sequence_create": (_int, [_vp, _u32, _u32, _u32, ctypes.POINTER(_vp)] + err),
         "q4b_sequence_add_matmul": (_int, [_vp, ctypes.POINTER(_vp), _int, _vp, ctypes.POINTER(_vp),
                                            ctypes.POINTER(_u32), _int] + err),
@@ -489,6 +525,32 @@ class Q4Context:
         """fp16 x of a layer's matmuls from its hidden state (q4b_rmsnorm)."""
         self._check(library().q4b_rmsnorm(self.handle, input_ptr, input_dtype, weight_ptr, output_ptr, hidden,
                                           batch_rows, epsilon, self._err, _ERR))
+
+    def rope_append(self, cache: KVCache, batch: TokenBatch, rope: Rope, q_ptr: int, k_ptr: int, v_ptr: int, dtype: int,
+                    q_heads: int, q_out_ptr: int, ldq: int | None = None, q_head_stride: int | None = None,
+                    ldk: int | None = None, ldv: int | None = None, ldq_out: int | None = None):
+        """Rotated k and v into the paged cache, rotated q to q_out (q4b_rope_append); strides default to dense rows."""
+        head = cache.head_size
+        self._check(library().q4b_rope_append(
+            self.handle, cache, batch, rope, q_ptr, q_heads * head if ldq is None else ldq,
+            head if q_head_stride is None else q_head_stride, k_ptr, cache.kv_heads * head if ldk is None else ldk, v_ptr,
+            cache.kv_heads * head if ldv is None else ldv, dtype, q_heads, q_out_ptr,
+            q_heads * head if ldq_out is None else ldq_out, self._err, _ERR))
+
+    def attention(self, cache: KVCache, batch: TokenBatch, q_ptr: int, q_heads: int, out_ptr: int, scale: float,
+                  window: int = 0, sinks: int = 0, ldq: int | None = None, ldo: int | None = None):
+        """Causal attention of the batch's tokens over the paged cache (q4b_attention)."""
+        width = q_heads * cache.head_size
+        self._check(library().q4b_attention(self.handle, cache, batch, q_ptr, width if ldq is None else ldq, q_heads, scale,
+                                            window, sinks, out_ptr, width if ldo is None else ldo, self._err, _ERR))
+
+    def sample(self, logits_ptr: int, dtype: int, rows: int, vocab: int, uniform_ptr: int, tokens_ptr: int,
+               temperature: int | None = None, top_k: int | None = None, top_p: int | None = None, min_p: int | None = None,
+               probability_ptr: int | None = None, ld: int | None = None):
+        """One token per row of logits (q4b_sample); the rules are device pointers, None is off."""
+        rules = Sampling(temperature, top_k, top_p, min_p)
+        self._check(library().q4b_sample(self.handle, logits_ptr, dtype, rows, vocab, vocab if ld is None else ld, rules,
+                                         uniform_ptr, tokens_ptr, probability_ptr, self._err, _ERR))
 
     def gate_up_silu(self, gate: Q4Weight, up: Q4Weight, x_ptr: int, x_dtype: int, m_rows: int, y_ptr: int,
                      y_dtype: int = F16, ldy: int | None = None):

@@ -243,6 +243,93 @@ int q4b_weight_rows(const q4b_weight *weight, uint32_t row_begin, uint32_t row_c
 int q4b_matmul_rows(q4b_context *context, const q4b_weight *weight, const uint32_t *row_ids, uint32_t count,
                     const void *x, int x_dtype, uint32_t m_rows, void *y, int y_dtype, uint32_t ldy,
                     char *error_message, size_t error_capacity);
+/* ---- between a layer's projections: the paged cache and attention over it (the place of the rotation, cache
+ * store and GQA decode kernels that the reference encodes between encode_attention's two projections,
+ * qwen38_m3_decode.m:747-795; the paged form, ragged batches, windows and sinks have no counterpart there).
+ *
+ * q4b_kv_cache names one layer's cache: two pools of pages in DEVICE memory, each [pages][kv_heads][page_tokens]
+ * [head_size], fp16 or bf16, 16-byte aligned.  page_tokens is a power of two from 16 to 1024, head_size 64, 128
+ * or 256.  q4b_token_batch names the tokens of one call: rows [token_begin[s], token_begin[s+1]) of q, k, v and
+ * the outputs belong to sequence s and are its last tokens, in order; lengths[s] counts all its tokens INCLUDING
+ * these; token j of it lives in page page_table[s * table_stride + j / page_tokens] at place j % page_tokens.
+ * token_begin [sequences + 1], lengths [sequences] and page_table are DEVICE memory, read when the kernels run, so
+ * a recorded call (q4b_graph_begin) sees what they hold at each replay.  tokens is the number of rows that the
+ * buffers hold; rows behind token_begin[sequences] are left as they are.  most_tokens (0: unknown) is the most rows
+ * that any one sequence brings: it chooses a kernel and changes no result beyond rounding.  The structures
+ * themselves are HOST memory and only read during the call.
+ *
+ * What the device finds wrong in them (a page that the pool does not have, a table too short for a length,
+ * token_begin that falls or passes `tokens`) is skipped, never followed, and reported by the next q4b_sync with
+ * status 1; the outputs of that call are then not to be used. */
+typedef struct {
+    void *keys, *values;
+    int dtype; /* Q4B_F16 or Q4B_BF16 */
+    uint32_t pages, page_tokens, kv_heads, head_size;
+} q4b_kv_cache;
+typedef struct {
+    uint32_t sequences, tokens, most_tokens;
+    const uint32_t *token_begin, *lengths, *page_table;
+    uint32_t table_stride;
+} q4b_token_batch;
+/* Rotation: value pairs of the first rotary_size values of a head (a multiple of 16, 0 to head_size) turn by
+ * position * frequency(i), i = 0 .. rotary_size/2 - 1; the rest passes through.  Pairs are (i, i + rotary_size/2)
+ * (HALVES, the reference's form) or (2i, 2i + 1) (NEIGHBOURS).  frequency(i) = base^(-2i / rotary_size), or
+ * frequencies[i] where that HOST array is given (scaled forms).  The position is the token's place in its sequence, or
+ * positions[row] where that DEVICE array is given.  Angles are reduced in 64 bits: positions of millions keep fp32's
+ * accuracy. */
+enum { Q4B_ROPE_HALVES = 0, Q4B_ROPE_NEIGHBOURS = 1 };
+typedef struct {
+    uint32_t rotary_size;
+    int pairing;
+    double base;
+    const double *frequencies;
+    const int32_t *positions;
+} q4b_rope;
+/* Rotates q and k, writes k and v into the cache and the rotated q to q_out (the cache's type), one launch.  q is
+ * [tokens][ldq] with head h at h * q_head_stride (so a projection that interleaves q with something else is read in
+ * place), k and v [tokens][ldk], [tokens][ldv] with heads next to each other; q, k and v share dtype (fp16, fp32 or
+ * bf16) and may be columns of one matrix.  q_out is [tokens][ldq_out], heads next to each other; it may be q itself
+ * when dtype, head stride and row stride agree, and must not overlap it otherwise.  Strides count values; pointers are
+ * 16-byte aligned and strides whole multiples of 16 bytes.  Computed in fp32, rounded once.  A token whose place in
+ * its sequence is negative (lengths[s] smaller than its rows: left padding) is skipped.  Two tokens of one call that
+ * share a slot leave either one's values in it.  Asynchronous. */
+int q4b_rope_append(q4b_context *context, const q4b_kv_cache *cache, const q4b_token_batch *batch, const q4b_rope *rope,
+                    const void *q, uint32_t ldq, uint32_t q_head_stride, const void *k, uint32_t ldk, const void *v,
+                    uint32_t ldv, int dtype, uint32_t q_heads, void *q_out, uint32_t ldq_out,
+                    char *error_message, size_t error_capacity);
+/* Causal attention of the batch's tokens over the cache: a token at place p sees the cached tokens j <= p, with a
+ * window (window > 0) only those with j > p - window or j < sinks.  out[row][h] = sum_j softmax_j(scale * q[row][h] .
+ * key[j][h / group]) value[j][h / group], group = q_heads / kv_heads.  q is [tokens][ldq], out [tokens][ldo], heads
+ * next to each other, both in the cache's type; pointers 16-byte aligned, strides multiples of 8 values.  out must not
+ * overlap q.  Scores, maxima, sums and the output's accumulation are fp32; a weight is rounded to the cache's type
+ * before it meets the values.  A row that sees nothing (p < 0) is zeros.  What is not visible has no influence,
+ * whatever it holds, infinities and NaN included.  The result does not depend on timing.  The first call on a context
+ * allocates a workspace (never while recording).  Asynchronous. */
+int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_token_batch *batch, const void *q,
+                  uint32_t ldq, uint32_t q_heads, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
+                  char *error_message, size_t error_capacity);
+/* ---- behind the lm_head: one token per row of logits [rows][ld] (fp32, fp16 or bf16) from a given random number
+ * (the place of the reference's sampler, qwen38_sampler.c, which picks on the CPU).  The rules are DEVICE arrays
+ * [rows], any of them NULL (off):
+ *   temperature  weights are exp((logit - largest) / temperature); <= 0 is greedy: the largest logit, the lowest
+ *                index among equals, probability 1, the other rules unused; NULL is 1
+ *   top_k        only the k largest logits, the lowest index first among equals; 0 is off
+ *   top_p        of these the fewest, largest first, whose weights reach top_p of their sum (at least one); >= 1 is off
+ *   min_p        of these those whose weight is at least min_p of the largest one's; <= 0 is off, above 1 counts as 1
+ * A NaN in temperature is greedy, one in top_p or min_p is off, one in uniform is 0.
+ * The token is the first one, in index order, at which the running sum of the kept weights exceeds uniform[row] (in
+ * [0, 1)) times their sum.  tokens [rows] and, if not NULL, probabilities [rows] (the token's share among the kept)
+ * are written.  A NaN logit counts as -infinity; several logits of +infinity share everything; a row with nothing above
+ * -infinity gives token 0xffffffff and probability 0.  Sums are exact integers of weights in units of 2^-42, so a
+ * result depends on nothing but its row.  vocab is 1 .. 2^20; logits are aligned to their type.  Asynchronous. */
+typedef struct {
+    const float *temperature;
+    const uint32_t *top_k;
+    const float *top_p, *min_p;
+} q4b_sampling;
+int q4b_sample(q4b_context *context, const void *logits, int dtype, uint32_t rows, uint32_t vocab, uint32_t ld,
+               const q4b_sampling *rules, const float *uniform, uint32_t *tokens, float *probabilities,
+               char *error_message, size_t error_capacity);
 /* Up to 4 matrices that share x in one launch, e.g. q/k/v, which the reference
  * fuses into one matrix (qwen38_attention.metal:4-8). */
 int q4b_matmul_group(q4b_context *context, const q4b_weight *const *weights, int count,
