@@ -576,6 +576,8 @@ size_t attention_partial_bytes(int sm_count) {
 size_t attention_arrival_bytes(int sm_count) { return (size_t)sm_count * kBlocksPerSm * sizeof(uint32_t); }
 
 cudaError_t launch_attention(const AttentionArgs &args, int sm_count, cudaStream_t stream) {
+    const uint64_t rows = (uint64_t)(args.most_tokens != 0 ? args.most_tokens : args.batch.tokens) * args.group;
+    if (rows > kMostRows && prompt_serves(args)) return launch_prompt(args, sm_count, stream);
     return args.cache.dtype == kBF16 ? launch_head<__nv_bfloat16>(args, sm_count, stream)
                                      : launch_head<__half>(args, sm_count, stream);
 }

@@ -41,24 +41,25 @@ __host__ __device__ inline SequenceRows sequence_rows(const BatchView &batch, ui
 
 constexpr uint32_t kGroupKeys = 16;  // keys that attention takes together: the rows of one matrix product
 
-// The groups of 16 keys that a run of rows of one sequence may see: [0, sink_groups) and [first, end).
+// The groups of keys that a run of rows of one sequence may see: [0, sink) and [first, end).
 struct Groups {
     uint32_t sink, first, end;
     __host__ __device__ inline uint32_t count() const { return sink + (end - first) == 0 ? 1u : sink + (end - first); }  // an empty unit still answers
     __host__ __device__ inline uint32_t at(uint32_t i) const { return i < sink ? i : first + (i - sink); }
 };
 // rows from token `token0` to `token1` (inclusive) of the sequence's new ones
+template <uint32_t KEYS = kGroupKeys>
 __host__ __device__ inline Groups groups_of(const SequenceRows &rows, uint32_t token0, uint32_t token1, uint32_t window,
-                                   uint32_t sinks) {
+                                            uint32_t sinks) {
     Groups g;
     const int64_t low = (int64_t)rows.length - rows.count + token0, high = (int64_t)rows.length - rows.count + token1;
-    g.end = high < 0 ? 0u : (uint32_t)(high / kGroupKeys) + 1;
+    g.end = high < 0 ? 0u : (uint32_t)(high / KEYS) + 1;
     g.first = 0;
     g.sink = 0;
     if (window != 0 && low - (int64_t)window + 1 > 0) {
-        const uint32_t first = (uint32_t)((low - (int64_t)window + 1) / kGroupKeys);
+        const uint32_t first = (uint32_t)((low - (int64_t)window + 1) / KEYS);
         g.first = first < g.end ? first : g.end;
-        const uint32_t sink = (uint32_t)(((uint64_t)sinks + kGroupKeys - 1) / kGroupKeys);
+        const uint32_t sink = (uint32_t)(((uint64_t)sinks + KEYS - 1) / KEYS);
         g.sink = sink < g.first ? sink : g.first;
     }
     return g;

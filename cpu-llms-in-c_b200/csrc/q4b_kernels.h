@@ -171,6 +171,9 @@ struct AttentionArgs {
 size_t attention_partial_bytes(int sm_count);
 size_t attention_arrival_bytes(int sm_count);
 cudaError_t launch_attention(const AttentionArgs &args, int sm_count, cudaStream_t stream);
+// ---- q4b_prompt.cu: the same for many rows per sequence, on tcgen05 ----
+bool prompt_serves(const AttentionArgs &args);
+cudaError_t launch_prompt(const AttentionArgs &args, int sm_count, cudaStream_t stream);
 
 // ---- q4b_sample.cu ----
 struct SampleArgs {

@@ -1,0 +1,668 @@
+// Attention of many new tokens per sequence over the paged cache (prompts, pieces of prompts, wide verify steps).
+//
+//   out(t, h) = sum_j w_j v(j) / sum_j w_j,   w_j = exp(scale q(t, h) . k(j) - m)
+//
+// The tensor cores' share is 4 D multiplications per visible (query head, key) pair, so the kernel is bound by them and
+// by what feeds them.  A unit is 128 query rows of one key head -- (token, query head of the group) pairs, tokens
+// outside -- so a key head's keys and values are read once for all its query heads.  Per tile of 128 keys:
+//   S[128 x 128] = Q K^T   tcgen05.mma, both operands in shared memory (128-byte swizzle), S in TMEM, two buffers
+//   P = exp2(S c - m)      eight warps, two threads per row of 64 columns each; 16-bit P goes back over S in TMEM
+//   O[128 x D] += P V      tcgen05.mma, P from TMEM, V as it lies in the cache (rows of keys: the MN-major form)
+// TMEM: O takes D columns, S 2 x 128: 512 at D = 256.  The order on the tensor pipe is S(0) S(1) | O(0) S(2) | O(1) S(3)
+// ...: while the warps turn S(j+1) into P(j+1), the pipe does O(j) and S(j+2).
+//
+// The running maximum is moved only when a row's grows by more than 2^8: weights then stay below 256 (exact enough in 16
+// bits, sums are fp32), and O in TMEM is rescaled a few times per unit instead of once per tile.
+//
+// Keys and values come by TMA straight from their pages, a box of at most 64 tokens x 64 columns each, through one ring
+// that both share in the order in which they are used; a ring slot is 128 keys x D/2 columns or 64 keys x D columns.
+// Tiles on the edge of what the rows see are masked, and their values are looked at first by two warps of their own: what
+// lies behind the sequence's end becomes zero, and an infinity or a NaN (0 x infinity would reach rows that must
+// not see it) sends the unit through a plain fp32 loop at the end.
+//
+// When there are fewer units than SMs the keys of a unit are split over a cluster of 2 to 8 thread blocks, whose sums meet
+// in distributed shared memory.
+#include "q4b_cache.cuh"
+#include "q4b_tc.cuh"
+
+#include <cooperative_groups.h>
+#include <cmath>
+#include <type_traits>
+
+namespace q4b {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr uint32_t kPromptThreads = 384;   // producer, MMA, two that look at values, eight of the softmax
+constexpr uint32_t kTileRowsQ = 128, kTileKeys = 128;
+constexpr uint32_t kMostSplits = 8;
+constexpr float kRescaleAt = 8.0f;         // powers of two
+
+template <int D> struct Shape {
+    static constexpr uint32_t parts = D == 64 ? 1 : 2;              // ring slots of a tile of keys, or of values
+    static constexpr uint32_t slot = kTileKeys * D * 2 / parts;
+    static constexpr uint32_t slots = D == 256 ? 5 : 10;
+    static constexpr uint32_t chunks = D / 64;                      // 128-byte columns
+    static constexpr uint32_t query = kTileRowsQ * D * 2;
+};
+constexpr uint32_t kMiscBytes = 2048;
+
+struct PromptParams {
+    CUtensorMap k_map, v_map;   // [pages x kv_heads x page_tokens][D], box 64 columns x box_rows
+    AttentionArgs a;
+    uint32_t units, splits, box_rows;
+};
+
+__device__ inline float exp2_of(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+template <typename T> __device__ inline uint32_t pack2(float low, float high);
+template <> __device__ inline uint32_t pack2<__half>(float low, float high) {
+    const __half2 h = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+template <> __device__ inline uint32_t pack2<__nv_bfloat16>(float low, float high) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(low, high);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ inline float wide(__half x) { return __half2float(x); }
+__device__ inline float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ inline void pair_barrier(uint32_t id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// What a thread block works on.
+struct Unit {
+    SequenceRows rows;
+    uint32_t sequence, head, row0, count;  // query rows [row0, row0 + count) of the sequence's count x group
+    Groups tiles;                          // of 128 keys
+    uint32_t first, size;                  // this thread block's share of them
+    int64_t least, most, place0;           // places of the first and the last row; of the sequence's first new token
+    __device__ inline uint32_t key(uint32_t j) const { return tiles.at(first + j) * kTileKeys; }
+    __device__ inline bool clear(const AttentionArgs &a, uint32_t key0) const {
+        return (int64_t)key0 + kTileKeys - 1 <= least &&
+               (a.window == 0 || (int64_t)key0 > most - (int64_t)a.window || (uint64_t)key0 + kTileKeys <= a.sinks);
+    }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kPromptThreads, 1)
+prompt_kernel(const __grid_constant__ PromptParams p) {
+    using S = Shape<D>;
+    extern __shared__ __align__(1024) uint8_t prompt_smem[];
+    uint8_t *const base = prompt_smem + ((1024u - (tc_smem_u32(prompt_smem) & 1023u)) & 1023u);
+    uint8_t *const query = base, *const ring = base + S::query;
+    uint8_t *const misc = ring + S::slots * S::slot;
+    float *const exchange = reinterpret_cast<float *>(misc);                    // [2][128]
+    uint64_t *const bars = reinterpret_cast<uint64_t *>(misc + 1024);
+    uint32_t *const words = reinterpret_cast<uint32_t *>(bars + 2 * S::slots + 8);  // TMEM address, poison flag
+    const uint32_t full0 = tc_smem_u32(bars), empty0 = full0 + 8 * S::slots;
+    const uint32_t q_full = empty0 + 8 * S::slots, s_full0 = q_full + 8, p_full0 = s_full0 + 16, o_done = p_full0 + 16,
+                   v_look = o_done + 8, v_ready = v_look + 8;
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const AttentionArgs &a = p.a;
+    const uint32_t rank = blockIdx.x % p.splits;
+
+    // ---- which rows ---- (the last tiles of a sequence see most: they go first)
+    Unit u;
+    {
+        const uint32_t index = p.units - 1 - blockIdx.x / p.splits;
+        u.head = index % a.cache.kv_heads;
+        const uint32_t tile = index / a.cache.kv_heads;
+        uint32_t before = 0;
+        bool found = false;
+        for (uint32_t s0 = 0; s0 < a.batch.sequences && !found; s0 += 32) {
+            uint32_t own = 0;
+            if (s0 + lane < a.batch.sequences)
+                own = ceil_div(sequence_rows(a.batch, a.cache.page_tokens, s0 + lane, a.status).count * a.group, kTileRowsQ);
+            uint32_t inclusive = own;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, inclusive, d);
+                if (lane >= (uint32_t)d) inclusive += y;
+            }
+            const uint32_t passed = __ballot_sync(0xffffffffu, before + inclusive > tile);
+            if (passed != 0) {
+                const int at = __ffs(passed) - 1;
+                u.sequence = s0 + at;
+                u.row0 = (tile - before - __shfl_sync(0xffffffffu, inclusive - own, at)) * kTileRowsQ;
+                found = true;
+            }
+            before += __shfl_sync(0xffffffffu, inclusive, 31);
+        }
+        if (!found) return;  // the grid is made for the most tiles that the host's numbers allow; the whole cluster leaves
+        u.rows = sequence_rows(a.batch, a.cache.page_tokens, u.sequence, a.status);
+        u.count = min(kTileRowsQ, u.rows.count * a.group - u.row0);
+        const uint32_t token0 = u.row0 / a.group, token1 = (u.row0 + u.count - 1) / a.group;
+        u.tiles = groups_of<kTileKeys>(u.rows, token0, token1, a.window, a.sinks);
+        u.place0 = (int64_t)u.rows.length - u.rows.count;
+        u.least = u.place0 + token0;
+        u.most = u.place0 + token1;
+        const uint32_t all = u.tiles.sink + (u.tiles.end - u.tiles.first);
+        u.first = (uint32_t)((uint64_t)all * rank / p.splits);
+        u.size = (uint32_t)((uint64_t)all * (rank + 1) / p.splits) - u.first;
+    }
+    const uint32_t n = u.size;
+    const uint32_t *const table = a.batch.table + (size_t)u.sequence * a.batch.table_stride;
+
+    if (threadIdx.x == 0) {
+        for (uint32_t s = 0; s < S::slots; ++s) {
+            tc_mbar_init(full0 + 8 * s, 1);
+            tc_mbar_init(empty0 + 8 * s, 1);
+        }
+        tc_mbar_init(q_full, kPromptThreads - 64);
+        for (uint32_t b = 0; b < 2; ++b) {
+            tc_mbar_init(s_full0 + 8 * b, 1);
+            tc_mbar_init(p_full0 + 8 * b, 8);
+        }
+        tc_mbar_init(o_done, 1);
+        tc_mbar_init(v_look, 1);
+        tc_mbar_init(v_ready, 64);
+        words[1] = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(tc_smem_u32(words)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = words[0], tmem_o = tmem, tmem_s = tmem + 256;
+    bool ok = true;
+
+    if (warp == 0) {
+        // ---- producer: K(0) K(1) V(0) K(2) V(1) ... V(n-2) V(n-1), `parts` ring slots each ----
+        const uint32_t keys_end = u.rows.length;
+        uint32_t item = 0;
+        for (uint32_t order = 0; order < 2 * n && ok; ++order) {
+            const bool is_key = order == 0 || ((order & 1) && order != 2 * n - 1);
+            const uint32_t j = order == 0 ? 0 : order == 2 * n - 1 ? n - 1 : is_key ? (order + 1) / 2 : order / 2 - 1;
+            const uint32_t key0 = u.key(j);
+            for (uint32_t part = 0; part < S::parts && ok; ++part, ++item) {
+                // one box per lane: tokens outside, chunks of 64 columns inside
+                const uint32_t chunks = is_key ? S::chunks / S::parts : S::chunks;
+                const uint32_t rows = is_key ? kTileKeys : kTileKeys / S::parts;
+                const uint32_t boxes = rows / p.box_rows * chunks;
+                const uint32_t box = lane / chunks, chunk = lane % chunks;
+                const uint32_t token = key0 + (is_key ? 0 : part * rows) + box * p.box_rows;
+                bool present = lane < boxes && token < keys_end;
+                uint32_t page = 0;
+                if (present) {
+                    page = __ldg(table + (token >> a.cache.page_shift));
+                    if (page >= a.cache.pages) {
+                        report(a.status, kBadPage);
+                        present = false;
+                    }
+                }
+                const uint32_t slot = item % S::slots;
+                if (item >= S::slots && !tc_wait(empty0 + 8 * slot, ((item / S::slots) - 1) & 1)) ok = false;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const uint32_t count = __popc(__ballot_sync(0xffffffffu, present));
+                const uint32_t bar = full0 + 8 * slot;
+                if (lane == 0) tc_mbar_expect_tx(bar, count * p.box_rows * 128);
+                __syncwarp();
+                if (present) {
+                    const int x = (int)((is_key ? part * chunks + chunk : chunk) * 64);
+                    const int y = (int)((page * a.cache.kv_heads + u.head) * a.cache.page_tokens +
+                                        (token & (a.cache.page_tokens - 1)));
+                    tc_tensor_copy_2d(tc_smem_u32(ring) + slot * S::slot + (chunk * rows + box * p.box_rows) * 128,
+                                      is_key ? &p.k_map : &p.v_map, x, y, bar);
+                }
+            }
+        }
+        if (!ok) {
+            if (lane == 0) atomicExch(a.status, 0x81u);
+            // copies already issued land before the shared memory is released
+            for (uint32_t back = 0; back < S::slots && back < item; ++back) {
+                const uint32_t i = item - 1 - back;
+                tc_wait(full0 + 8 * (i % S::slots), (i / S::slots) & 1);
+            }
+        }
+    } else if (warp == 1) {
+        // ---- MMA issuer ----
+        if (lane == 0 && n > 0) {
+            constexpr uint32_t format = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
+            constexpr uint32_t s_idesc = (1u << 4) | format | ((kTileKeys >> 3) << 17) | ((128u >> 4) << 24);
+            constexpr uint32_t o_idesc = (1u << 4) | format | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
+            // rows of 128 bytes, eight of them 1024 bytes (stride field), swizzled; for V the 64-column chunks of a slot
+            // follow one another at the leading field's distance
+            constexpr uint64_t k_desc = ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+            constexpr uint64_t v_desc = ((uint64_t)((kTileKeys / S::parts) * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+                                        ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+            auto at = [](uint32_t address) { return (uint64_t)((address >> 4) & 0x3fffu); };
+            uint32_t item = 0, looked = 0;
+            auto scores = [&](uint32_t j) {
+#pragma unroll
+                for (uint32_t part = 0; part < S::parts; ++part, ++item) {
+                    const uint32_t slot = item % S::slots;
+                    if (!ok || !tc_wait(full0 + 8 * slot, (item / S::slots) & 1)) { ok = false; return; }
+                    tc_fence_after();
+                    const uint32_t keys = tc_smem_u32(ring) + slot * S::slot;
+                    const uint32_t rows = tc_smem_u32(query) + part * (S::chunks / S::parts) * (kTileRowsQ * 128);
+#pragma unroll
+                    for (uint32_t k = 0; k < D / 16 / S::parts; ++k) {
+                        const uint32_t offset = (k / 4) * (128 * 128) + (k % 4) * 32;
+                        tc_mma_shared(tmem_s + (j & 1) * 128, k_desc | at(rows + offset), k_desc | at(keys + offset), s_idesc,
+                                      part > 0 || k > 0 ? 1u : 0u);
+                    }
+                    tc_commit(empty0 + 8 * slot);
+                }
+                tc_commit(s_full0 + 8 * (j & 1));
+            };
+            if (!tc_wait(q_full, 0)) ok = false;
+            tc_fence_after();
+            scores(0);
+            if (n > 1) scores(1);
+            for (uint32_t j = 0; j < n && ok; ++j) {
+                // a masked tile's values are handed to the two warps that look at them and handed back: a strict exchange,
+                // so neither side can miss a round of a barrier that the other is already past
+                const bool edge = !u.clear(a, u.key(j));
+                if (edge) {
+                    for (uint32_t part = 0; part < S::parts && ok; ++part)
+                        if (!tc_wait(full0 + 8 * ((item + part) % S::slots), ((item + part) / S::slots) & 1)) ok = false;
+                    if (!ok) break;
+                    tc_mbar_arrive(v_look);
+                }
+                if (!tc_wait(p_full0 + 8 * (j & 1), (j >> 1) & 1)) { ok = false; break; }
+                if (edge) {
+                    if (!tc_wait(v_ready, looked & 1)) { ok = false; break; }
+                    ++looked;
+                }
+                tc_fence_after();
+#pragma unroll
+                for (uint32_t part = 0; part < S::parts && ok; ++part, ++item) {
+                    const uint32_t slot = item % S::slots;
+                    if (!tc_wait(full0 + 8 * slot, (item / S::slots) & 1)) { ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t values = tc_smem_u32(ring) + slot * S::slot;
+#pragma unroll
+                    for (uint32_t k = 0; k < kTileKeys / 16 / S::parts; ++k) {
+                        tc_mma(tmem_o, tmem_s + (j & 1) * 128 + (part * (kTileKeys / 16 / S::parts) + k) * 8,
+                               v_desc | at(values + k * 16 * 128), o_idesc, j > 0 || part > 0 || k > 0 ? 1u : 0u);
+                    }
+                    tc_commit(empty0 + 8 * slot);
+                }
+                if (!ok) break;
+                tc_commit(o_done);
+                if (j + 2 < n) scores(j + 2);
+            }
+            if (!ok) atomicExch(a.status, 0x82u);
+        }
+    } else {
+        // ---- query rows into shared memory, swizzled; a negative scale turns their sign, scale 0 makes them zero ----
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, hold = a.scale == 0.0f ? 0u : 0xffffffffu;
+        for (uint32_t i = threadIdx.x - 64; i < kTileRowsQ * (D / 8); i += kPromptThreads - 64) {
+            const uint32_t row = i / (D / 8), piece = i % (D / 8);
+            uint4 value = make_uint4(0, 0, 0, 0);
+            if (row < u.count) {
+                const uint32_t flat = u.row0 + row;
+                value = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
+                                                         (size_t)(u.rows.begin + flat / a.group) * a.ldq +
+                                                         (size_t)(u.head * a.group + flat % a.group) * D + piece * 8);
+                value = make_uint4((value.x ^ flip) & hold, (value.y ^ flip) & hold, (value.z ^ flip) & hold, (value.w ^ flip) & hold);
+            }
+            *reinterpret_cast<uint4 *>(query + (piece >> 3) * (kTileRowsQ * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16)) = value;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        tc_mbar_arrive(q_full);
+
+        if (warp < 4) {
+            // ---- the values of masked tiles: zeros behind the sequence's end, and no infinity among the rest ----
+            const uint32_t thread = threadIdx.x - 64;
+            constexpr uint32_t exponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+            uint32_t looked = 0;
+            for (uint32_t j = 0; j < n && ok; ++j) {
+                const uint32_t key0 = u.key(j);
+                if (u.clear(a, key0)) continue;
+                if (!tc_wait(v_look, looked & 1)) { ok = false; break; }
+                ++looked;
+                const uint32_t item0 = min(2 * j + 2, 2 * n - 1) * S::parts;
+                uint32_t strange = 0;
+                for (uint32_t part = 0; part < S::parts && ok; ++part) {
+                    const uint32_t slot = (item0 + part) % S::slots;
+                    if (!tc_wait(full0 + 8 * slot, ((item0 + part) / S::slots) & 1)) { ok = false; break; }  // it is: acquires
+                    constexpr uint32_t rows = kTileKeys / S::parts;
+                    const uint32_t held = key0 + part * rows < u.rows.length ? min(rows, u.rows.length - key0 - part * rows) : 0;
+                    uint4 *const cells = reinterpret_cast<uint4 *>(ring + slot * S::slot);
+#pragma unroll 8
+                    for (uint32_t i = thread; i < S::slot / 16; i += 64) {
+                        if (((i >> 3) & (rows - 1)) >= held) {
+                            cells[i] = make_uint4(0, 0, 0, 0);
+                        } else {
+                            const uint4 c = cells[i];
+                            // an exponent of all ones carries into the bit above it
+                            constexpr uint32_t both = exponent | exponent << 16, low = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+                            strange |= (((c.x & both) + low) | ((c.y & both) + low) | ((c.z & both) + low) | ((c.w & both) + low)) & 0x80008000u;
+                        }
+                    }
+                }
+                if (strange != 0) words[1] = 1;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                tc_mbar_arrive(v_ready);
+            }
+            if (!ok && lane == 0) atomicExch(a.status, 0x83u);
+        } else {
+            // ---- softmax ----
+            const uint32_t quad = warp & 3, half = (warp - 4) >> 2, row = quad * 32 + lane;
+            const uint32_t lanes = (quad * 32) << 16;
+            const float c = a.scale == 0.0f ? 1.0f : fabsf(a.scale) * 1.44269504088896341f;
+            const bool active = quad * 32 < u.count;  // otherwise none of the warp's rows is asked for
+            const int64_t place = row < u.count ? u.place0 + (u.row0 + row) / a.group : -1;
+            float top = -INFINITY, total = 0.0f;
+            for (uint32_t j = 0; j < n; ++j) {
+                if (ok && !tc_wait(s_full0 + 8 * (j & 1), (j >> 1) & 1)) ok = false;
+                tc_fence_after();
+                const uint32_t s_columns = tmem_s + (j & 1) * 128 + lanes;
+                if (active) {
+                    uint32_t raw[2][32];
+                    tc_load_32(s_columns + half * 64, raw[0]);
+                    tc_load_32(s_columns + half * 64 + 32, raw[1]);
+                    tc_wait_load();
+                    const uint32_t key0 = u.key(j);
+                    if (!u.clear(a, key0)) {
+                        // visible columns: below `high`, and from `low` on or below `sink`
+                        const int64_t first = (int64_t)key0 + half * 64;
+                        const int32_t high = (int32_t)max((int64_t)0, min((int64_t)64, place + 1 - first));
+                        const int32_t low = a.window == 0 ? 0 : (int32_t)max((int64_t)0, min((int64_t)64, place - (int64_t)a.window + 1 - first));
+                        const int32_t sink = (int32_t)max((int64_t)0, min((int64_t)64, (int64_t)a.sinks - first));
+#pragma unroll
+                        for (int i = 0; i < 64; ++i) {
+                            if (!(i < high && (i >= low || i < sink))) raw[i >> 5][i & 31] = 0xff800000u;  // -infinity
+                        }
+                    }
+                    float high = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) high = fmaxf(high, __uint_as_float(raw[i >> 5][i & 31]));
+                    pair_barrier(5 + quad);  // the other half has read what it was told last time
+                    exchange[half * 128 + row] = high;
+                    pair_barrier(1 + quad);
+                    high = fmaxf(high, exchange[(half ^ 1) * 128 + row]) * c;
+                    const bool grow = high > top + kRescaleAt || (top == -INFINITY && high > -INFINITY);
+                    bool waited = j == 0;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float factor = grow ? exp2_of(top - high) : 1.0f;
+                        if (grow) top = high;
+                        total *= factor;
+                        if (j > 0) {
+                            if (ok && !tc_wait(o_done, (j - 1) & 1)) ok = false;
+                            waited = true;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (uint32_t column = half * (D / 2); column < (half + 1) * (D / 2); column += 32) {
+                                uint32_t o[32];
+                                tc_load_32(tmem_o + lanes + column, o);
+                                tc_wait_load();
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                                tc_store_32(tmem_o + lanes + column, o);
+                            }
+                        }
+                    }
+                    const float minus = top == -INFINITY ? 0.0f : -top;
+                    uint32_t weights[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const float x = exp2_of(fmaf(__uint_as_float(raw[i >> 4][(2 * i) & 31]), c, minus));
+                        const float y = exp2_of(fmaf(__uint_as_float(raw[i >> 4][(2 * i + 1) & 31]), c, minus));
+                        total += x + y;
+                        weights[i] = pack2<T>(x, y);
+                    }
+                    tc_store_32(s_columns + half * 32, weights);
+                    tc_wait_store();
+                    // O(j - 1) is complete long before P(j) is needed; every warp sees every round of its barrier
+                    if (!waited && ok && !tc_wait(o_done, (j - 1) & 1)) ok = false;
+                } else if (j > 0 && ok && !tc_wait(o_done, (j - 1) & 1)) {
+                    ok = false;
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) tc_mbar_arrive(p_full0 + 8 * (j & 1));
+            }
+            if (n > 0 && ok && !tc_wait(o_done, (n - 1) & 1)) ok = false;
+            if (!ok && lane == 0) atomicExch(a.status, 0x84u);
+            tc_fence_after();
+            if (active) {
+                pair_barrier(5 + quad);
+                exchange[half * 128 + row] = total;
+                pair_barrier(1 + quad);
+                total = exchange[row] + exchange[128 + row];
+            }
+            // ---- output, or sums for the cluster ----
+            const uint32_t flat = u.row0 + row;
+            if (p.splits == 1) {
+                const float over = total == 0.0f ? 0.0f : 1.0f / total;
+                if (active) {
+#pragma unroll 1
+                    for (uint32_t column = half * (D / 2); column < (half + 1) * (D / 2); column += 32) {
+                        uint32_t o[32];
+                        if (n > 0) {
+                            tc_load_32(tmem_o + lanes + column, o);
+                            tc_wait_load();
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = 0;
+                        }
+                        if (row < u.count) {
+                            T *to = static_cast<T *>(a.out) + (size_t)(u.rows.begin + flat / a.group) * a.ldo +
+                                    (size_t)(u.head * a.group + flat % a.group) * D + column;
+#pragma unroll
+                            for (int i = 0; i < 32; i += 8) {
+                                uint4 packed;
+                                uint32_t *const w = reinterpret_cast<uint32_t *>(&packed);
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    w[k] = pack2<T>(__uint_as_float(o[i + 2 * k]) * over, __uint_as_float(o[i + 2 * k + 1]) * over);
+                                *reinterpret_cast<uint4 *>(to + i) = packed;
+                            }
+                        }
+                    }
+                }
+            } else if (active) {
+                float *const sums = reinterpret_cast<float *>(ring);  // [128][D], pieces of four turned by the row
+#pragma unroll 1
+                for (uint32_t column = half * (D / 2); column < (half + 1) * (D / 2); column += 32) {
+                    uint32_t o[32];
+                    if (n > 0) {
+                        tc_load_32(tmem_o + lanes + column, o);
+                        tc_wait_load();
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = 0;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        *reinterpret_cast<uint4 *>(sums + row * D + (((column + i) / 4) ^ (row & 7)) * 4) =
+                            make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    }
+                }
+                pair_barrier(5 + quad);  // both have read the totals
+                if (half == 0) {
+                    exchange[row] = top;
+                    exchange[128 + row] = total;
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) {
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
+    }
+
+    // ---- a unit whose edge tiles hold infinities or NaN: again, row by row in fp32, over what each row sees ----
+    if (words[1] != 0) {
+        float *const sums = reinterpret_cast<float *>(ring);
+        for (uint32_t row = warp; row < u.count; row += kPromptThreads / 32) {
+            const uint32_t flat = u.row0 + row;
+            const int64_t place = u.place0 + flat / a.group;
+            const T *const q = static_cast<const T *>(a.q) + (size_t)(u.rows.begin + flat / a.group) * a.ldq +
+                               (size_t)(u.head * a.group + flat % a.group) * D;
+            float mine[D / 32], sum[D / 32], top = -INFINITY, total = 0.0f;
+#pragma unroll
+            for (int i = 0; i < D / 32; ++i) {
+                mine[i] = wide(q[i * 32 + lane]) * a.scale * 1.44269504088896341f;
+                sum[i] = 0.0f;
+            }
+            for (uint32_t j = 0; j < n; ++j) {
+                for (uint32_t key = u.key(j); key < u.key(j) + kTileKeys; ++key) {
+                    if ((int64_t)key > place || !(a.window == 0 || (int64_t)key > place - (int64_t)a.window || key < a.sinks)) continue;
+                    const uint32_t page = __ldg(table + (key >> a.cache.page_shift));
+                    if (page >= a.cache.pages) continue;
+                    const size_t line = (((size_t)page * a.cache.kv_heads + u.head) * a.cache.page_tokens +
+                                         (key & (a.cache.page_tokens - 1))) * D;
+                    float score = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) score += mine[i] * wide(static_cast<const T *>(a.cache.keys)[line + i * 32 + lane]);
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) score += __shfl_xor_sync(0xffffffffu, score, d);
+                    const float high = fmaxf(top, score);
+                    const float minus = high == -INFINITY ? 0.0f : high;
+                    const float keep = exp2_of(top - minus), weight = exp2_of(score - minus);
+                    top = high;
+                    total = total * keep + weight;
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i)
+                        sum[i] = sum[i] * keep + weight * wide(static_cast<const T *>(a.cache.values)[line + i * 32 + lane]);
+                }
+            }
+            if (p.splits == 1) {
+                T *const to = static_cast<T *>(a.out) + (size_t)(u.rows.begin + flat / a.group) * a.ldo +
+                              (size_t)(u.head * a.group + flat % a.group) * D;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const uint32_t word = pack2<T>(total == 0.0f ? 0.0f : sum[i] / total, 0.0f);
+                    to[i * 32 + lane] = *reinterpret_cast<const T *>(&word);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) {
+                    const uint32_t column = i * 32 + lane;
+                    sums[row * D + ((column / 4) ^ (row & 7)) * 4 + (column & 3)] = sum[i];
+                }
+                if (lane == 0) {
+                    exchange[row] = top;
+                    exchange[128 + row] = total;
+                }
+            }
+        }
+    }
+    if (p.splits > 1) {
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        // the rows are dealt to the cluster's warps; sums are added in the order of the split
+        for (uint32_t row = rank + p.splits * warp; row < u.count; row += p.splits * (kPromptThreads / 32)) {
+            float high = -INFINITY;
+            for (uint32_t r = 0; r < p.splits; ++r) high = fmaxf(high, cluster.map_shared_rank(exchange, r)[row]);
+            float total = 0.0f;
+            float4 sum[D > 128 ? D / 128 : 1];
+#pragma unroll
+            for (int i = 0; i < (D > 128 ? D / 128 : 1); ++i) sum[i] = make_float4(0, 0, 0, 0);
+            for (uint32_t r = 0; r < p.splits; ++r) {
+                const float *const told = cluster.map_shared_rank(exchange, r);
+                const float factor = told[row] == -INFINITY ? 1.0f : exp2_of(told[row] - high);
+                total += told[128 + row] * factor;
+                const float *const sums = reinterpret_cast<const float *>(cluster.map_shared_rank(ring, r)) + row * D;
+#pragma unroll
+                for (int i = 0; i < (D > 128 ? D / 128 : 1); ++i) {
+                    if (D >= 128 || lane < D / 4) {
+                        const float4 part = *reinterpret_cast<const float4 *>(sums + ((i * 32 + lane) ^ (row & 7)) * 4);
+                        sum[i].x += part.x * factor; sum[i].y += part.y * factor;
+                        sum[i].z += part.z * factor; sum[i].w += part.w * factor;
+                    }
+                }
+            }
+            const float over = total == 0.0f ? 0.0f : 1.0f / total;
+            const uint32_t flat = u.row0 + row;
+            T *const to = static_cast<T *>(a.out) + (size_t)(u.rows.begin + flat / a.group) * a.ldo +
+                          (size_t)(u.head * a.group + flat % a.group) * D;
+#pragma unroll
+            for (int i = 0; i < (D > 128 ? D / 128 : 1); ++i) {
+                if (D >= 128 || lane < D / 4)
+                    *reinterpret_cast<uint2 *>(to + (i * 32 + lane) * 4) =
+                        make_uint2(pack2<T>(sum[i].x * over, sum[i].y * over), pack2<T>(sum[i].z * over, sum[i].w * over));
+            }
+        }
+        cluster.sync();  // the sums stay until everybody has read them
+    }
+}
+
+template <typename T, int D>
+cudaError_t launch_prompt_of(const AttentionArgs &args, int sm_count, cudaStream_t stream) {
+    using S = Shape<D>;
+    EncodeTiledFn encode = encode_tiled();
+    if (encode == nullptr) return cudaErrorNotSupported;
+    PromptParams p;
+    p.a = args;
+    p.box_rows = args.cache.page_tokens < 64 ? args.cache.page_tokens : 64;
+    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)args.cache.pages * args.cache.kv_heads * args.cache.page_tokens};
+    const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+    const cuuint32_t box[2] = {64, p.box_rows};
+    const cuuint32_t element_strides[2] = {1, 1};
+    const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    for (int which = 0; which < 2; ++which) {
+        if (encode(which == 0 ? &p.k_map : &p.v_map, type, 2, which == 0 ? args.cache.keys : args.cache.values, dims, strides, box,
+                   element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return cudaErrorInvalidValue;
+    }
+    // as many tiles of rows as the host's numbers allow: full ones, and one ragged one per sequence
+    const uint64_t tiles = (uint64_t)args.batch.tokens * args.group / kTileRowsQ +
+                           (args.batch.sequences < args.batch.tokens ? args.batch.sequences : args.batch.tokens);
+    const uint64_t units = tiles * args.cache.kv_heads;
+    p.splits = 1;
+    while (p.splits < kMostSplits && units * (p.splits + 1) <= (uint64_t)sm_count) ++p.splits;
+    if (units * p.splits > 0x7fffffffu) return cudaErrorInvalidConfiguration;
+    p.units = (uint32_t)units;
+    const size_t smem = S::query + (size_t)S::slots * S::slot + kMiscBytes + 1024;
+    static bool configured[kMaxDevices] = {};
+    const int slot = device_slot();
+    if (slot < 0 || !configured[slot]) {
+        cudaError_t status = cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (status != cudaSuccess) return status;
+        if (slot >= 0) configured[slot] = true;
+    }
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)(units * p.splits));
+    config.blockDim = dim3(kPromptThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = p.splits;
+    attribute[0].val.clusterDim.y = 1;
+    attribute[0].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    return cudaLaunchKernelEx(&config, prompt_kernel<T, D>, p);
+}
+
+template <typename T>
+cudaError_t launch_prompt_head(const AttentionArgs &args, int sm_count, cudaStream_t stream) {
+    switch (args.cache.head_size) {
+        case 64: return launch_prompt_of<T, 64>(args, sm_count, stream);
+        case 128: return launch_prompt_of<T, 128>(args, sm_count, stream);
+        case 256: return launch_prompt_of<T, 256>(args, sm_count, stream);
+    }
+    return cudaErrorInvalidValue;
+}
+
+}  // namespace
+
+bool prompt_serves(const AttentionArgs &args) {
+    // TMA counts the pools' rows in 31 bits
+    return (uint64_t)args.cache.pages * args.cache.kv_heads * args.cache.page_tokens <= 0x7fffffffull;
+}
+
+cudaError_t launch_prompt(const AttentionArgs &args, int sm_count, cudaStream_t stream) {
+    return args.cache.dtype == kBF16 ? launch_prompt_head<__nv_bfloat16>(args, sm_count, stream)
+                                     : launch_prompt_head<__half>(args, sm_count, stream);
+}
+
+}  // namespace q4b

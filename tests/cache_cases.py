@@ -80,16 +80,18 @@ def attention_reference(batch, q, q_heads, scale, window, sinks):
     tolerance = np.full_like(out, np.nan)
     keys, values, q = widen(batch.keys, batch.dtype), widen(batch.values, batch.dtype), widen(q, batch.dtype)
     for s in range(len(batch.counts)):
+        held = batch.table[s, :-(-int(batch.lengths[s]) // batch.page)].astype(np.int64)
+        own_keys = keys[held].transpose(1, 0, 2, 3).reshape(batch.kv_heads, -1, head)      # [kv_heads, places, head]
+        own_values = values[held].transpose(1, 0, 2, 3).reshape(batch.kv_heads, -1, head)
         for i in range(int(batch.counts[s])):
             row, at = int(batch.begin[s]) + i, batch.place(s, i)
-            seen = [j for j in range(at + 1) if window == 0 or j > at - window or j < sinks]
+            every = np.arange(at + 1)
+            seen = every[(every > at - window) | (every < sinks)] if window else every
             out[row] = tolerance[row] = 0.0
-            if not seen:
+            if len(seen) == 0:
                 continue
-            slots = [batch.slot(s, j) for j in seen]
             for h in range(batch.kv_heads):
-                k = np.stack([keys[page, h, place] for page, place in slots])
-                v = np.stack([values[page, h, place] for page, place in slots])
+                k, v = own_keys[h, seen], own_values[h, seen]
                 x = q[row].reshape(batch.kv_heads, group, head)[h]
                 score = x @ k.T * scale
                 error = abs(scale) * (np.abs(x) @ np.abs(k).T).max(axis=1) * (head + 8) * 2.0 ** -24 * 2

@@ -81,6 +81,36 @@ def test_a_long_context_is_split_and_joined(q4b, ctx, page):
     check(q4b, ctx, batch, 4)
 
 
+@pytest.mark.parametrize("dtype,head,page,kv_heads,group,counts,lengths,window,sinks", [
+    ("f16", 256, 64, 2, 6, [500], [2300], 0, 0), ("bf16", 128, 16, 2, 4, [700, 33], [701, 1400], 0, 0),
+    ("f16", 64, 32, 1, 8, [400], [5000], 0, 0), ("bf16", 256, 16, 2, 8, [900], [900], 300, 5),
+    ("f16", 128, 128, 1, 5, [7, 300], [4000, 2000], 1000, 200), ("bf16", 64, 1024, 4, 1, [777], [777], 0, 0),
+    ("f16", 256, 16, 1, 24, [1, 2], [3000, 1000], 0, 0), ("bf16", 256, 32, 1, 6, [4, 4, 4], [2000, 3, 900], 512, 4)])
+def test_prompts_and_pieces_of_prompts(q4b, ctx, dtype, head, page, kv_heads, group, counts, lengths, window, sinks):
+    """Many tiles of rows and of keys: rings and barriers go round, keys are split over clusters or are not."""
+    rng = np.random.default_rng(head + page)
+    batch = Batch(rng, counts, lengths, page, kv_heads, head, dtype, pad=2)
+    check(q4b, ctx, batch, kv_heads * group, window, sinks)
+
+
+def test_growing_scores(q4b, ctx):
+    """Keys whose scores grow along the sequence: the running maximum is passed again and again."""
+    rng = np.random.default_rng(8)
+    for head in (64, 128, 256):
+        batch = Batch(rng, [60], [1500], 32, 1, head, "f16")
+        ramp = np.zeros(batch.stride * batch.page)
+        ramp[:1500] = np.linspace(0, 1, 1500)
+        direction = rng.choice([-1.0, 1.0], size=head)
+        for j in range(1500):
+            page, place = batch.slot(0, j)
+            batch.keys[page, 0, place] = narrow(direction * ramp[j] * 2 + rng.standard_normal(head) * 0.1, "f16")
+        q = narrow(np.broadcast_to(direction, (batch.tokens, 4, head)) * 2.0 + rng.standard_normal((batch.tokens, 4, head)) * 0.1, "f16")
+        for scale in (0.3, -0.3):
+            got = widen(attend(q4b, ctx, batch, q, 4, scale, 0, 0), "f16")
+            want, tolerance = attention_reference(batch, q, 4, scale, 0, 0)
+            assert (np.abs(got - want) <= tolerance).all()
+
+
 def test_many_unlike_sequences(q4b, ctx):
     rng = np.random.default_rng(5)
     lengths = rng.integers(1, 90, size=300)
