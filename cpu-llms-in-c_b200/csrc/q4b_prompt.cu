@@ -14,11 +14,12 @@
 // The running maximum is moved only when a row's grows by more than 2^8: weights then stay below 256 (exact enough in 16
 // bits, sums are fp32), and O in TMEM is rescaled a few times per unit instead of once per tile.
 //
-// Keys and values come by TMA straight from their pages, a box of at most 64 tokens x 64 columns each, through one ring
-// that both share in the order in which they are used; a ring slot is 128 keys x D/2 columns or 64 keys x D columns.
-// Tiles on the edge of what the rows see are masked, and their values are looked at first by two warps of their own: what
-// lies behind the sequence's end becomes zero, and an infinity or a NaN (0 x infinity would reach rows that must
-// not see it) sends the unit through a plain fp32 loop at the end.
+// Keys and values come by TMA straight from their pages, through a ring and a producer warp of their own each: a slot of
+// 16 KB is 128 keys x 64 columns, or the values of 8192 / D keys.  A copy costs its warp about 60 clocks however small it
+// is, and a slot's barriers as much again; one warp for both was the bound of the whole kernel (3,700 clocks per tile).
+// Tiles on the edge of what the rows see are masked, and their values are looked at first by a warp of its own: what no
+// row sees becomes zero, and an infinity or a NaN that some rows see and others do not (0 x infinity is NaN) sends the
+// unit through a plain fp32 loop at the end.
 //
 // When there are fewer units than SMs the keys of a unit are split over a cluster of 2 to 8 thread blocks, whose sums meet
 // in distributed shared memory.
@@ -40,19 +41,19 @@ constexpr uint32_t kTileRowsQ = 128, kTileKeys = 128;
 constexpr uint32_t kMostSplits = 8;
 constexpr float kRescaleAt = 8.0f;         // powers of two
 
+constexpr uint32_t kSlotBytes = 16384;
 template <int D> struct Shape {
-    static constexpr uint32_t parts = D == 64 ? 1 : 2;              // ring slots of a tile of keys, or of values
-    static constexpr uint32_t slot = kTileKeys * D * 2 / parts;
-    static constexpr uint32_t slots = D == 256 ? 5 : 10;
-    static constexpr uint32_t chunks = D / 64;                      // 128-byte columns
+    static constexpr uint32_t parts = D / 64;                       // ring slots of a tile of keys, or of values
+    static constexpr uint32_t slots = D == 256 ? 5 : 6;             // of either ring
+    static constexpr uint32_t v_rows = kTileKeys / parts;           // a slot is 128 keys x 64 columns, or v_rows values x D
     static constexpr uint32_t query = kTileRowsQ * D * 2;
 };
 constexpr uint32_t kMiscBytes = 2048;
 
 struct PromptParams {
-    CUtensorMap k_map, v_map;   // [pages x kv_heads x page_tokens][D], box 64 columns x box_rows
+    CUtensorMap k_map, v_map;   // [D / 64][pages x kv_heads x page_tokens][64]
     AttentionArgs a;
-    uint32_t units, splits, box_rows;
+    uint32_t units, splits, k_shift, v_shift;  // boxes of 1 << k_shift, 1 << v_shift tokens
 };
 
 __device__ inline float exp2_of(float x) {
@@ -94,12 +95,14 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     extern __shared__ __align__(1024) uint8_t prompt_smem[];
     uint8_t *const base = prompt_smem + ((1024u - (tc_smem_u32(prompt_smem) & 1023u)) & 1023u);
     uint8_t *const query = base, *const ring = base + S::query;
-    uint8_t *const misc = ring + S::slots * S::slot;
+    uint8_t *const misc = ring + 2 * S::slots * kSlotBytes;
     float *const exchange = reinterpret_cast<float *>(misc);                    // [2][128]
     uint64_t *const bars = reinterpret_cast<uint64_t *>(misc + 1024);
-    uint32_t *const words = reinterpret_cast<uint32_t *>(bars + 2 * S::slots + 8);  // TMEM address, poison flag
-    const uint32_t full0 = tc_smem_u32(bars), empty0 = full0 + 8 * S::slots;
-    const uint32_t q_full = empty0 + 8 * S::slots, s_full0 = q_full + 8, p_full0 = s_full0 + 16, o_done = p_full0 + 16,
+    uint32_t *const words = reinterpret_cast<uint32_t *>(bars + 4 * S::slots + 8);  // TMEM address, poison flag
+    const uint32_t k_full0 = tc_smem_u32(bars), k_empty0 = k_full0 + 8 * S::slots, v_full0 = k_empty0 + 8 * S::slots,
+                   v_empty0 = v_full0 + 8 * S::slots;
+    const uint32_t k_ring = tc_smem_u32(ring), v_ring = k_ring + S::slots * kSlotBytes;
+    const uint32_t q_full = v_empty0 + 8 * S::slots, s_full0 = q_full + 8, p_full0 = s_full0 + 16, o_done = p_full0 + 16,
                    v_look = o_done + 8, v_ready = v_look + 8;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const AttentionArgs &a = p.a;
@@ -148,18 +151,15 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     const uint32_t *const table = a.batch.table + (size_t)u.sequence * a.batch.table_stride;
 
     if (threadIdx.x == 0) {
-        for (uint32_t s = 0; s < S::slots; ++s) {
-            tc_mbar_init(full0 + 8 * s, 1);
-            tc_mbar_init(empty0 + 8 * s, 1);
-        }
-        tc_mbar_init(q_full, kPromptThreads - 64);
+        for (uint32_t s = 0; s < 4 * S::slots; ++s) tc_mbar_init(k_full0 + 8 * s, 1);  // full and empty of both rings
+        tc_mbar_init(q_full, kPromptThreads - 96);
         for (uint32_t b = 0; b < 2; ++b) {
             tc_mbar_init(s_full0 + 8 * b, 1);
             tc_mbar_init(p_full0 + 8 * b, 8);
         }
         tc_mbar_init(o_done, 1);
         tc_mbar_init(v_look, 1);
-        tc_mbar_init(v_ready, 64);
+        tc_mbar_init(v_ready, 32);
         words[1] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -175,49 +175,56 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     const uint32_t tmem = words[0], tmem_o = tmem, tmem_s = tmem + 256;
     bool ok = true;
 
-    if (warp == 0) {
-        // ---- producer: K(0) K(1) V(0) K(2) V(1) ... V(n-2) V(n-1), `parts` ring slots each ----
-        const uint32_t keys_end = u.rows.length;
-        uint32_t item = 0;
-        for (uint32_t order = 0; order < 2 * n && ok; ++order) {
-            const bool is_key = order == 0 || ((order & 1) && order != 2 * n - 1);
-            const uint32_t j = order == 0 ? 0 : order == 2 * n - 1 ? n - 1 : is_key ? (order + 1) / 2 : order / 2 - 1;
-            const uint32_t key0 = u.key(j);
-            for (uint32_t part = 0; part < S::parts && ok; ++part, ++item) {
-                // one box per lane: tokens outside, chunks of 64 columns inside
-                const uint32_t chunks = is_key ? S::chunks / S::parts : S::chunks;
-                const uint32_t rows = is_key ? kTileKeys : kTileKeys / S::parts;
-                const uint32_t boxes = rows / p.box_rows * chunks;
-                const uint32_t box = lane / chunks, chunk = lane % chunks;
-                const uint32_t token = key0 + (is_key ? 0 : part * rows) + box * p.box_rows;
-                bool present = lane < boxes && token < keys_end;
-                uint32_t page = 0;
-                if (present) {
-                    page = __ldg(table + (token >> a.cache.page_shift));
-                    if (page >= a.cache.pages) {
-                        report(a.status, kBadPage);
-                        present = false;
-                    }
+    if (warp == 0 || warp == 2) {
+        // ---- producers: warp 0 the keys, warp 2 the values ----
+        // A box ends with its page.  Page numbers are fetched, one box per lane, a whole tile ahead of their use.
+        const bool keys = warp == 0;
+        const uint32_t keys_end = u.rows.length, shift = keys ? p.k_shift : p.v_shift;
+        const uint32_t rows = keys ? kTileKeys : S::v_rows, box_bytes = (keys ? 128u : 128u * S::parts) << shift;
+        const uint32_t full0 = keys ? k_full0 : v_full0, empty0 = keys ? k_empty0 : v_empty0, to0 = keys ? k_ring : v_ring;
+        const CUtensorMap *const map = keys ? &p.k_map : &p.v_map;
+        const uint32_t my_token = min(lane << shift, kTileKeys - 1);
+        // the token of this lane's box; one behind the sequence's end counts as the last one (its box is not fetched)
+        auto token_of = [&](uint32_t j) { return min(u.key(j) + my_token, keys_end - 1); };
+        auto page_of = [&](uint32_t token) { return __ldg(table + (token >> a.cache.page_shift)); };
+        const bool leader = tc_leader();
+        uint32_t item = 0, slot = 0, lap = 0;
+        uint32_t token = n > 0 ? token_of(0) : 0, page = n > 0 ? page_of(token) : 0;
+        for (uint32_t j = 0; j < n && ok; ++j) {
+            const uint32_t held = min(kTileKeys, keys_end - u.key(j));
+            if (page >= a.cache.pages) {  // never followed: the pool's first page stands in for it
+                report(a.status, kBadPage);
+                page = 0;
+            }
+            const int line = (int)((page * a.cache.kv_heads + u.head) * a.cache.page_tokens + (token & (a.cache.page_tokens - 1)));
+            if (j + 1 < n) {
+                token = token_of(j + 1);
+                page = page_of(token);
+            }
+#pragma unroll
+            for (uint32_t part = 0; part < S::parts; ++part) {
+                if (lap > 0 && !tc_warp_wait(empty0 + 8 * slot, (lap - 1) & 1)) {
+                    ok = false;
+                    break;
                 }
-                const uint32_t slot = item % S::slots;
-                if (item >= S::slots && !tc_wait(empty0 + 8 * slot, ((item / S::slots) - 1) & 1)) ok = false;
-                ok = __all_sync(0xffffffffu, ok);
-                if (!ok) break;
-                const uint32_t count = __popc(__ballot_sync(0xffffffffu, present));
+                const uint32_t first = keys ? 0 : part * S::v_rows;
+                const uint32_t boxes = first >= held ? 0 : (min(rows, held - first) + (1u << shift) - 1) >> shift;
                 const uint32_t bar = full0 + 8 * slot;
-                if (lane == 0) tc_mbar_expect_tx(bar, count * p.box_rows * 128);
+                uint32_t to = to0 + slot * kSlotBytes;
+                if (leader) tc_mbar_expect_tx(bar, boxes * box_bytes);
                 __syncwarp();
-                if (present) {
-                    const int x = (int)((is_key ? part * chunks + chunk : chunk) * 64);
-                    const int y = (int)((page * a.cache.kv_heads + u.head) * a.cache.page_tokens +
-                                        (token & (a.cache.page_tokens - 1)));
-                    tc_tensor_copy_2d(tc_smem_u32(ring) + slot * S::slot + (chunk * rows + box * p.box_rows) * 128,
-                                      is_key ? &p.k_map : &p.v_map, x, y, bar);
+                for (uint32_t box = 0; box < boxes; ++box, to += box_bytes)
+                    tc_tensor_copy_3d_by(leader, to, map, 0, __shfl_sync(0xffffffffu, line, (first >> shift) + box),
+                                         keys ? (int)part : 0, bar);
+                ++item;
+                if (++slot == S::slots) {
+                    slot = 0;
+                    ++lap;
                 }
             }
         }
         if (!ok) {
-            if (lane == 0) atomicExch(a.status, 0x81u);
+            if (leader) atomicExch(a.status, keys ? 0x81u : 0x85u);
             // copies already issued land before the shared memory is released
             for (uint32_t back = 0; back < S::slots && back < item; ++back) {
                 const uint32_t i = item - 1 - back;
@@ -226,78 +233,91 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
         }
     } else if (warp == 1) {
         // ---- MMA issuer ----
-        if (lane == 0 && n > 0) {
+        if (n > 0) {
             constexpr uint32_t format = std::is_same<T, __nv_bfloat16>::value ? (1u << 7) | (1u << 10) : 0u;
             constexpr uint32_t s_idesc = (1u << 4) | format | ((kTileKeys >> 3) << 17) | ((128u >> 4) << 24);
             constexpr uint32_t o_idesc = (1u << 4) | format | (1u << 16) | (((uint32_t)D >> 3) << 17) | ((128u >> 4) << 24);
-            // rows of 128 bytes, eight of them 1024 bytes (stride field), swizzled; for V the 64-column chunks of a slot
+            // rows of 128 bytes, eight of them 1024 bytes (stride field), swizzled; for V the 64-column chunks of a box
             // follow one another at the leading field's distance
             constexpr uint64_t k_desc = ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-            constexpr uint64_t v_desc = ((uint64_t)((kTileKeys / S::parts) * 128 >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-                                        ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+            const uint64_t v_desc = ((uint64_t)((128u << p.v_shift) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+                                    ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
             auto at = [](uint32_t address) { return (uint64_t)((address >> 4) & 0x3fffu); };
-            uint32_t item = 0, looked = 0;
+            const bool leader = tc_leader();
+            const uint32_t to_s = __shfl_sync(0xffffffffu, tmem_s, 0), to_o = __shfl_sync(0xffffffffu, tmem_o, 0);
+            const uint32_t rows0 = tc_smem_u32(query);
+            uint32_t k_slot = 0, k_lap = 0, v_slot = 0, v_lap = 0, looked = 0;
+            auto advance = [](uint32_t &slot, uint32_t &lap) {
+                if (++slot == S::slots) {
+                    slot = 0;
+                    ++lap;
+                }
+            };
             auto scores = [&](uint32_t j) {
 #pragma unroll
-                for (uint32_t part = 0; part < S::parts; ++part, ++item) {
-                    const uint32_t slot = item % S::slots;
-                    if (!ok || !tc_wait(full0 + 8 * slot, (item / S::slots) & 1)) { ok = false; return; }
+                for (uint32_t part = 0; part < S::parts; ++part) {
+                    if (!tc_warp_wait(k_full0 + 8 * k_slot, k_lap & 1)) return false;
                     tc_fence_after();
-                    const uint32_t keys = tc_smem_u32(ring) + slot * S::slot;
-                    const uint32_t rows = tc_smem_u32(query) + part * (S::chunks / S::parts) * (kTileRowsQ * 128);
+                    const uint32_t keys = k_ring + k_slot * kSlotBytes, rows = rows0 + part * (kTileRowsQ * 128);
 #pragma unroll
-                    for (uint32_t k = 0; k < D / 16 / S::parts; ++k) {
-                        const uint32_t offset = (k / 4) * (128 * 128) + (k % 4) * 32;
-                        tc_mma_shared(tmem_s + (j & 1) * 128, k_desc | at(rows + offset), k_desc | at(keys + offset), s_idesc,
-                                      part > 0 || k > 0 ? 1u : 0u);
-                    }
-                    tc_commit(empty0 + 8 * slot);
+                    for (uint32_t k = 0; k < 4; ++k)
+                        tc_mma_shared_by(leader, to_s + (j & 1) * 128, k_desc | at(rows + k * 32), k_desc | at(keys + k * 32), s_idesc,
+                                         part > 0 || k > 0 ? 1u : 0u);
+                    tc_commit_by(leader, k_empty0 + 8 * k_slot);
+                    advance(k_slot, k_lap);
                 }
-                tc_commit(s_full0 + 8 * (j & 1));
+                tc_commit_by(leader, s_full0 + 8 * (j & 1));
+                return true;
             };
-            if (!tc_wait(q_full, 0)) ok = false;
+            ok = tc_warp_wait(q_full, 0);
             tc_fence_after();
-            scores(0);
-            if (n > 1) scores(1);
+            if (ok) ok = scores(0);
+            if (ok && n > 1) ok = scores(1);
             for (uint32_t j = 0; j < n && ok; ++j) {
-                // a masked tile's values are handed to the two warps that look at them and handed back: a strict exchange,
+                // a masked tile's values are handed to the warp that looks at them and handed back: a strict exchange,
                 // so neither side can miss a round of a barrier that the other is already past
                 const bool edge = !u.clear(a, u.key(j));
                 if (edge) {
-                    for (uint32_t part = 0; part < S::parts && ok; ++part)
-                        if (!tc_wait(full0 + 8 * ((item + part) % S::slots), ((item + part) / S::slots) & 1)) ok = false;
+                    uint32_t slot = v_slot, lap = v_lap;
+#pragma unroll
+                    for (uint32_t part = 0; part < S::parts; ++part) {
+                        if (ok) ok = tc_warp_wait(v_full0 + 8 * slot, lap & 1);
+                        advance(slot, lap);
+                    }
                     if (!ok) break;
-                    tc_mbar_arrive(v_look);
+                    if (leader) tc_mbar_arrive(v_look);
                 }
-                if (!tc_wait(p_full0 + 8 * (j & 1), (j >> 1) & 1)) { ok = false; break; }
-                if (edge) {
-                    if (!tc_wait(v_ready, looked & 1)) { ok = false; break; }
+                ok = tc_warp_wait(p_full0 + 8 * (j & 1), (j >> 1) & 1);
+                if (edge && ok) {
+                    ok = tc_warp_wait(v_ready, looked & 1);
                     ++looked;
                 }
                 tc_fence_after();
 #pragma unroll
-                for (uint32_t part = 0; part < S::parts && ok; ++part, ++item) {
-                    const uint32_t slot = item % S::slots;
-                    if (!tc_wait(full0 + 8 * slot, (item / S::slots) & 1)) { ok = false; break; }
+                for (uint32_t part = 0; part < S::parts; ++part) {
+                    if (ok) ok = tc_warp_wait(v_full0 + 8 * v_slot, v_lap & 1);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t values = tc_smem_u32(ring) + slot * S::slot;
+                    const uint32_t values = v_ring + v_slot * kSlotBytes;
 #pragma unroll
-                    for (uint32_t k = 0; k < kTileKeys / 16 / S::parts; ++k) {
-                        tc_mma(tmem_o, tmem_s + (j & 1) * 128 + (part * (kTileKeys / 16 / S::parts) + k) * 8,
-                               v_desc | at(values + k * 16 * 128), o_idesc, j > 0 || part > 0 || k > 0 ? 1u : 0u);
+                    for (uint32_t k = 0; k < S::v_rows / 16; ++k) {
+                        tc_mma_by(leader, to_o, to_s + (j & 1) * 128 + (part * (S::v_rows / 16) + k) * 8,
+                                  v_desc | at(values + ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 128),
+                                  o_idesc, j > 0 || part > 0 || k > 0 ? 1u : 0u);
                     }
-                    tc_commit(empty0 + 8 * slot);
+                    tc_commit_by(leader, v_empty0 + 8 * v_slot);
+                    advance(v_slot, v_lap);
                 }
                 if (!ok) break;
-                tc_commit(o_done);
-                if (j + 2 < n) scores(j + 2);
+                tc_commit_by(leader, o_done);
+                if (j + 2 < n) ok = scores(j + 2);
             }
-            if (!ok) atomicExch(a.status, 0x82u);
+            if (!ok && leader) atomicExch(a.status, 0x82u);
         }
     } else {
         // ---- query rows into shared memory, swizzled; a negative scale turns their sign, scale 0 makes them zero ----
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, hold = a.scale == 0.0f ? 0u : 0xffffffffu;
-        for (uint32_t i = threadIdx.x - 64; i < kTileRowsQ * (D / 8); i += kPromptThreads - 64) {
+        for (uint32_t i = threadIdx.x - 96; i < kTileRowsQ * (D / 8); i += kPromptThreads - 96) {
             const uint32_t row = i / (D / 8), piece = i % (D / 8);
             uint4 value = make_uint4(0, 0, 0, 0);
             if (row < u.count) {
@@ -312,32 +332,33 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tc_mbar_arrive(q_full);
 
-        if (warp < 4) {
-            // ---- the values of masked tiles: zeros behind the sequence's end, and no infinity among the rest ----
-            const uint32_t thread = threadIdx.x - 64;
+        if (warp == 3) {
+            // ---- the values of masked tiles: zeros where no row sees them, no infinity where only some rows do ----
             constexpr uint32_t exponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+            constexpr uint32_t both = exponent | exponent << 16, low = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+            constexpr uint32_t part_shift = S::parts == 4 ? 2 : S::parts == 2 ? 1 : 0;
+            const int64_t window = a.window, sinks = a.sinks;
             uint32_t looked = 0;
             for (uint32_t j = 0; j < n && ok; ++j) {
                 const uint32_t key0 = u.key(j);
                 if (u.clear(a, key0)) continue;
                 if (!tc_wait(v_look, looked & 1)) { ok = false; break; }
                 ++looked;
-                const uint32_t item0 = min(2 * j + 2, 2 * n - 1) * S::parts;
                 uint32_t strange = 0;
                 for (uint32_t part = 0; part < S::parts && ok; ++part) {
-                    const uint32_t slot = (item0 + part) % S::slots;
-                    if (!tc_wait(full0 + 8 * slot, ((item0 + part) / S::slots) & 1)) { ok = false; break; }  // it is: acquires
-                    constexpr uint32_t rows = kTileKeys / S::parts;
-                    const uint32_t held = key0 + part * rows < u.rows.length ? min(rows, u.rows.length - key0 - part * rows) : 0;
-                    uint4 *const cells = reinterpret_cast<uint4 *>(ring + slot * S::slot);
-#pragma unroll 8
-                    for (uint32_t i = thread; i < S::slot / 16; i += 64) {
-                        if (((i >> 3) & (rows - 1)) >= held) {
+                    const uint32_t item = j * S::parts + part, slot = item % S::slots;
+                    if (!tc_wait(v_full0 + 8 * slot, (item / S::slots) & 1)) { ok = false; break; }  // it is: acquires
+                    uint4 *const cells = reinterpret_cast<uint4 *>(ring + (S::slots + slot) * kSlotBytes);
+#pragma unroll 4
+                    for (uint32_t i = lane; i < kSlotBytes / 16; i += 32) {
+                        // [box][chunk][token of the box][8 cells]
+                        const uint32_t token = (i >> (p.v_shift + 3 + part_shift) << p.v_shift) + ((i >> 3) & ((1u << p.v_shift) - 1));
+                        const int64_t key = (int64_t)key0 + part * S::v_rows + token;
+                        if (key > u.most || (window != 0 && key <= u.least - window && key >= sinks)) {
                             cells[i] = make_uint4(0, 0, 0, 0);
-                        } else {
-                            const uint4 c = cells[i];
+                        } else if (!(key <= u.least && (window == 0 || key > u.most - window || key < sinks))) {
                             // an exponent of all ones carries into the bit above it
-                            constexpr uint32_t both = exponent | exponent << 16, low = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
+                            const uint4 c = cells[i];
                             strange |= (((c.x & both) + low) | ((c.y & both) + low) | ((c.z & both) + low) | ((c.w & both) + low)) & 0x80008000u;
                         }
                     }
@@ -600,15 +621,21 @@ cudaError_t launch_prompt_of(const AttentionArgs &args, int sm_count, cudaStream
     if (encode == nullptr) return cudaErrorNotSupported;
     PromptParams p;
     p.a = args;
-    p.box_rows = args.cache.page_tokens < 64 ? args.cache.page_tokens : 64;
-    const cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)args.cache.pages * args.cache.kv_heads * args.cache.page_tokens};
-    const cuuint64_t strides[1] = {(cuuint64_t)D * 2};
-    const cuuint32_t box[2] = {64, p.box_rows};
-    const cuuint32_t element_strides[2] = {1, 1};
+    // a box ends with its page or its slot; K's hold one chunk of 64 columns, V's all of them
+    const uint32_t page = args.cache.page_tokens, v_rows = S::v_rows;
+    const uint32_t k_tokens = page < kTileKeys ? page : kTileKeys, v_tokens = page < v_rows ? page : v_rows;
+    p.k_shift = p.v_shift = 4;
+    while ((1u << p.k_shift) < k_tokens) ++p.k_shift;
+    while ((1u << p.v_shift) < v_tokens) ++p.v_shift;
+    const cuuint64_t dims[3] = {64, (cuuint64_t)args.cache.pages * args.cache.kv_heads * page, (cuuint64_t)S::parts};
+    const cuuint64_t strides[2] = {(cuuint64_t)D * 2, 128};
+    const cuuint32_t element_strides[3] = {1, 1, 1};
     const CUtensorMapDataType type = std::is_same<T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
     for (int which = 0; which < 2; ++which) {
-        if (encode(which == 0 ? &p.k_map : &p.v_map, type, 2, which == 0 ? args.cache.keys : args.cache.values, dims, strides, box,
-                   element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+        const cuuint32_t k_box[3] = {64, k_tokens, 1};
+        const cuuint32_t v_box[3] = {64, v_tokens, S::parts};
+        if (encode(which == 0 ? &p.k_map : &p.v_map, type, 3, which == 0 ? args.cache.keys : args.cache.values, dims, strides,
+                   which == 0 ? k_box : v_box, element_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
     }
@@ -620,7 +647,7 @@ cudaError_t launch_prompt_of(const AttentionArgs &args, int sm_count, cudaStream
     while (p.splits < kMostSplits && units * (p.splits + 1) <= (uint64_t)sm_count) ++p.splits;
     if (units * p.splits > 0x7fffffffu) return cudaErrorInvalidConfiguration;
     p.units = (uint32_t)units;
-    const size_t smem = S::query + (size_t)S::slots * S::slot + kMiscBytes + 1024;
+    const size_t smem = S::query + (size_t)2 * S::slots * kSlotBytes + kMiscBytes + 1024;
     static bool configured[kMaxDevices] = {};
     const int slot = device_slot();
     if (slot < 0 || !configured[slot]) {

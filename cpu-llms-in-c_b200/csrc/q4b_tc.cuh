@@ -99,12 +99,49 @@ __device__ inline void tc_load_32(uint32_t address, uint32_t (&r)[32]) {
 }
 __device__ inline void tc_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ inline void tc_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// D[tmem_d] (+)= A[desc] * B[desc], both operands in shared memory, M = 128, K = 16
-__device__ inline void tc_mma_shared(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+// Forms for a warp that stays together: every branch goes by a vote and every operand is the same in all lanes, so the
+// compiler keeps them in uniform registers; `leader` is true in the one lane that issues.
+__device__ inline bool tc_leader() {
+    uint32_t leads;
     asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(leads));
+    return leads != 0;
+}
+__device__ inline bool tc_warp_wait(uint32_t bar, uint32_t parity) {
+    if (__all_sync(0xffffffffu, tc_try_wait(bar, parity))) return true;
+    const long long start = clock64();
+    while (!__all_sync(0xffffffffu, tc_try_wait(bar, parity))) {
+        if (__any_sync(0xffffffffu, clock64() - start > kTcWaitLimit)) return false;
+    }
+    return true;
+}
+__device__ inline void tc_mma_shared_by(bool leader, uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"((uint32_t)leader)
+        : "memory");
+}
+__device__ inline void tc_mma_by(bool leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"((uint32_t)leader)
+        : "memory");
+}
+__device__ inline void tc_commit_by(bool leader, uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(bar), "r"((uint32_t)leader) : "memory");
+}
+__device__ inline void tc_tensor_copy_3d_by(bool leader, uint32_t destination, const CUtensorMap *map, int x, int y, int z,
+                                            uint32_t bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %6, 0;\n\t"
+        "@q cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}"
+        ::"r"(destination), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"((uint32_t)leader)
         : "memory");
 }
 
