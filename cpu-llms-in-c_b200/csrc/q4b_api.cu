@@ -1189,7 +1189,7 @@ int q4b_sample(q4b_context *context, const void *logits, int dtype, uint32_t row
         args.top_p = rules->top_p;
         args.min_p = rules->min_p;
     }
-    cudaError_t status = launch_sample(args, context->stream);
+    cudaError_t status = launch_sample(args, context->sm_count, context->stream);
     if (!context->capturing) ++context->launches;
     if (status != cudaSuccess) return device_failure(error_message, error_capacity, "sample launch", status);
     return Q4B_OK;

@@ -187,7 +187,7 @@ struct SampleArgs {
     uint32_t *tokens;
     float *probabilities;
 };
-cudaError_t launch_sample(const SampleArgs &args, cudaStream_t stream);
+cudaError_t launch_sample(const SampleArgs &args, int sm_count, cudaStream_t stream);
 
 // ---- q4b_gemm.cu: tcgen05 prefill GEMM ----
 struct TcGemmArgs {

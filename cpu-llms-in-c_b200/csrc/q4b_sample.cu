@@ -3,20 +3,27 @@
 // All three cuts keep a prefix of the order (largest logit first, the lowest index first among equals), so each is ONE
 // composite number c = (ordered bits of the logit, complement of the index): an element stays when its own composite is
 // at least the cut.  The token is then the first index at which the running sum of the kept weights
-// exp((logit - largest) / temperature) passes uniform x total.  No sort is needed.
+// exp((logit - largest) / temperature) passes uniform x total.  A row is never sorted.
 //
-// A row is spread over a cluster of 1 to 8 thread blocks that keep it in shared memory: it is read from HBM once,
-// every further pass runs on chip.
-//   load      the largest composite (greedy ends here) and the smallest finite logit
-//   top-k     counts in 2048 bins, linear in the distance to the largest logit (linear bins spread a row of logits
-//             evenly; bins of the float's own bits would put most of a row into a few and serialise the atomics); the
-//             bin that holds the k-th element is gathered and ranked.  A bin too full for that is cut into 2048 again,
-//             by composite, which differ in all elements, so equal logits end too
-//   top-p     the same with weights in the bins
-//   token     sums of kept weights per 256 indices, then within the 256 that the target falls into
-// Weights are 64-bit integers in units of 2^-42 of the largest one's: sums are exact, in any order of the atomics, so
-// equal inputs give equal tokens.  exp is taken in fp64: in fp32 the argument alone is off by 2^-24 x |logit - largest|,
-// and over a flat distribution of 250,000 tokens such errors move the border between neighbours visibly.
+// A row is spread over a cluster of 1 to 8 thread blocks.  Few rows are kept in shared memory after their one trip from
+// HBM; with many rows in flight the passes read them again from L2 instead, which leaves room for two thread blocks
+// per SM whose passes hide each other's waits (256 rows of 248,320 fp32 logits: XX us against YY us).
+//   extremes  the largest and the smallest finite logit (greedy ends here)
+//   counts    2048 bins, linear in the distance to the largest logit: linear bins spread a row evenly, where bins of
+//             the float's own bits would put most of it into a few and serialise the atomics.  With top-p alone the same
+//             pass adds up all weights
+//   few stay  (the usual case: the bins down to the border hold at most 2048 elements): these are gathered in the first
+//             block of the cluster, sorted there, and everything else happens in that block
+//   many stay the border's bin alone is gathered and ranked and gives the cut.  For top-p the counts only bracket the
+//             border (a bin's weights differ by a per cent); the bracket is binned once more, now by exact weights
+//   token     sums of kept weights per 128 words of the row, then within the one that the target falls into
+//   A rare rest (both cuts deep in the row, thousands of equal logits at a border) goes through find_cut, which cuts the
+//   span in question into 2048 again and again.
+// Weights are integers in units of 2^-42 of the largest one's: sums are exact in any order of the atomics, so equal
+// inputs give equal tokens.  What decides between neighbours of a border is the error of a running sum, so a weight is
+// made to 2^-31, not to fp32's 2^-24 (whose argument alone would be off by 2^-24 x distance): the distance and its product
+// with log2(e) / temperature as unevaluated pairs of floats, a table of 2^(-j / 256), a cubic for the rest.  In fp64
+// the same pass is bound by the fp64 pipe and takes twice as long.
 #include "q4b_kernels.h"
 
 #include <cooperative_groups.h>
@@ -28,33 +35,54 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t kSampleThreads = 1024;
+constexpr uint32_t kSampleThreads = 512;
 constexpr uint32_t kSampleWarps = kSampleThreads / 32;
-constexpr uint32_t kBins = 2048;
+constexpr uint32_t kBins = 2048;           // at most: 512 per block of the cluster, a thread each
 constexpr uint32_t kMostBlocks = 8;        // thread blocks of a row
-constexpr uint32_t kListed = 1024;         // elements of a bin that are ranked one against another
-constexpr uint32_t kTile = 256;            // indices per partial sum of the last pass
-constexpr uint32_t kSliceBytes = 160 * 1024;  // of a row that a thread block keeps in shared memory; longer ones are read again
-constexpr uint32_t kMostTiles = (1u << 20) / kTile;
-constexpr double kUnit = 4398046511104.0;  // 2^42
+constexpr uint32_t kListed = 2048;         // elements that one block puts in order
+constexpr uint32_t kTileRows4 = 4;         // 16-byte words of a tile: 4 per lane of a warp
+constexpr uint32_t kTileWords = 32 * kTileRows4;
+constexpr uint32_t kSliceBytes = 160 * 1024;  // of a row that a thread block may keep in shared memory
+constexpr uint64_t kOne = 1ull << 42;      // the largest logit's weight
 
 struct SampleShared {
-    uint64_t high[kMostBlocks];          // largest composite of every block's slice
-    float low[kMostBlocks];              // smallest finite logit
-    uint64_t part_count[kMostBlocks], part_mass[kMostBlocks];  // of every 256 bins, over the whole row
-    uint64_t before_count, before_mass;  // in front of the border bin
-    uint32_t border, border_count;
-    uint64_t span_low[kMostBlocks], span_high[kMostBlocks];    // composites of the border bin
-    uint64_t cut;
+    uint2 power[256];                      // 2^(-j / 256): in units of 2^-31 as an integer, and as a float's bits
+    float high[kMostBlocks], low[kMostBlocks];
     uint64_t total[kMostBlocks];
+    uint64_t parts[3][kMostBlocks];        // sums of the blocks' shares of the bins
     uint64_t warp_values[kSampleWarps];
-    float warp_low[kSampleWarps];
-    uint32_t listed;
-    uint64_t list[kListed];
-    uint64_t list_weight[kListed];
+    float warp_high[kSampleWarps], warp_low[kSampleWarps];
+    uint32_t first, listed, low_bin, high_bin, found_count, fine_bin, fine_count;
+    uint64_t found_before, cut;
+    uint64_t span_low[kMostBlocks], span_high[kMostBlocks];
     uint32_t count[kBins];
-    uint64_t mass[kBins];
+    union {
+        uint64_t list[kListed];            // composites
+        uint64_t mass[kBins];
+    };
+    uint64_t sums[kListed];
 };
+
+// 2^(-j / 256), by repeated multiplication in fp64 (256 roundings of 2^-53 each)
+struct PowerTable {
+    uint2 entry[256];
+};
+constexpr uint32_t float_bits(double x) {  // of 2^30 < x <= 2^31, rounded
+    if (x >= 2147483648.0) return (158u << 23);
+    return (157u << 23) | ((uint32_t)((x - 1073741824.0) / 128.0 + 0.5) & 0x7fffffu) +
+                              (((uint32_t)((x - 1073741824.0) / 128.0 + 0.5) >> 23) << 23);
+}
+constexpr PowerTable make_powers() {
+    PowerTable table = {};
+    double value = 2147483648.0;
+    for (int j = 0; j < 256; ++j) {
+        table.entry[j].x = (uint32_t)(value + 0.5);
+        table.entry[j].y = float_bits(value);
+        value *= 0.997296056085470126;  // 2^(-1 / 256)
+    }
+    return table;
+}
+__device__ const PowerTable kPowers = make_powers();
 
 __device__ inline float as_float(float x) { return x; }
 __device__ inline float as_float(__half x) { return __half2float(x); }
@@ -73,7 +101,7 @@ __device__ inline float logit_of(uint64_t c) {
 }
 __device__ inline uint32_t index_of(uint64_t c) { return ~(uint32_t)c; }
 
-template <typename V> __device__ inline V warp_sum(V x) {
+__device__ inline uint64_t warp_sum(uint64_t x) {
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
     return x;
@@ -86,69 +114,170 @@ __device__ inline uint64_t warp_max(uint64_t x) {
     }
     return x;
 }
+__device__ inline uint64_t warp_inclusive(uint64_t x) {
+    const uint32_t lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const uint64_t y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= (uint32_t)d) x += y;
+    }
+    return x;
+}
 // the same in every thread of the block; `scratch` is free again afterwards
 __device__ inline uint64_t block_max(uint64_t x, uint64_t *scratch) {
     x = warp_max(x);
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
     __syncthreads();
-    x = warp_max(scratch[threadIdx.x & 31]);
+    x = warp_max(scratch[threadIdx.x & (kSampleWarps - 1)]);
     __syncthreads();
     return x;
+}
+// sum over the block, and (in `before`) over the threads in front of this one
+__device__ inline uint64_t block_scan(uint64_t x, uint64_t *scratch, uint64_t &before) {
+    const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const uint64_t inclusive = warp_inclusive(x);
+    if (lane == 31) scratch[warp] = inclusive;
+    __syncthreads();
+    const uint64_t warps = warp_inclusive(lane < kSampleWarps ? scratch[lane] : 0);
+    const uint64_t total = __shfl_sync(0xffffffffu, warps, kSampleWarps - 1);
+    before = inclusive - x + (warp > 0 ? __shfl_sync(0xffffffffu, warps, warp - 1) : 0);
+    __syncthreads();
+    return total;
 }
 __device__ inline uint64_t block_sum(uint64_t x, uint64_t *scratch) {
-    x = warp_sum(x);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = warp_sum(scratch[threadIdx.x & 31]);
-    __syncthreads();
-    return x;
-}
-__device__ inline float block_min(float x, float *scratch) {
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) x = fminf(x, __shfl_xor_sync(0xffffffffu, x, d));
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
-    __syncthreads();
-    x = scratch[threadIdx.x & 31];
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) x = fminf(x, __shfl_xor_sync(0xffffffffu, x, d));
-    __syncthreads();
-    return x;
+    uint64_t before;
+    return block_scan(x, scratch, before);
 }
 
+// This block's part of the row: `head` single values up to a 16-byte boundary, whole words, `tail` single values.
 template <typename T>
 struct Slice {
-    const T *data;       // this block's part of the row, in shared memory or where it was
-    uint32_t begin, size;
+    const T *data;
+    uint32_t begin, size, head, words, tail;
+    static constexpr uint32_t kWord = 16 / sizeof(T);
     __device__ inline float at(uint32_t i) const { return tidy(as_float(data[i])); }
-};
-
-struct Weigh {
-    float high;
-    double over;  // 1 / temperature
-    __device__ inline double real(float x) const {
-        const double distance = (double)x - (double)high;
-        if (x == high) return 1.0;
-        return distance == -INFINITY ? 0.0 : exp(distance * over);
+    __device__ inline uint32_t tiles() const { return (words + kTileWords - 1) / kTileWords; }
+    __device__ inline void split(uint32_t skew) {
+        head = min(size, skew == 0 ? 0u : (16u - skew) / (uint32_t)sizeof(T));
+        words = (size - head) / kWord;
+        tail = size - head - words * kWord;
     }
-    static __device__ inline uint64_t units(double w) { return (uint64_t)(w * kUnit + 0.5); }
+    // f(value, index within the slice) for the values of one tile, as a warp.  One word's code, not sixteen: a pass is
+    // short, and the instructions of longer loops took more time to arrive than to run.
+    template <typename F> __device__ inline void tile(uint32_t t, F f) const {
+        const uint4 *const from = reinterpret_cast<const uint4 *>(data + head);
+        uint32_t w = t * kTileWords + (threadIdx.x & 31);
+        uint4 next = w < words ? from[w] : make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+        for (uint32_t r = 0; r < kTileRows4; ++r, w += 32) {
+            const uint4 word = next;
+            if (r + 1 < kTileRows4 && w + 32 < words) next = from[w + 32];
+            if (w < words) {
+                const T *x = reinterpret_cast<const T *>(&word);
+#pragma unroll
+                for (uint32_t j = 0; j < kWord; ++j) f(tidy(as_float(x[j])), head + w * kWord + j);
+            }
+        }
+    }
+    // f over the whole slice, as a block; warp 0 has the head, warp 1 the tail
+    template <typename F> __device__ inline void each(F f) const {
+        const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 1
+        for (uint32_t t = warp; t < tiles(); t += kSampleWarps) tile(t, f);
+        if (warp == 0 && lane < head + tail) {
+            const uint32_t i = lane < head ? lane : size - tail + (lane - head);
+            f(at(i), i);
+        }
+    }
 };
 
-// Where the border lies: the composite of the last element that stays, over the whole cluster.  By count: the
-// `wanted`-th element of those at or above `floor`.  By mass: the first at which the running weight reaches `wanted`.
+// Weights by the distance to the largest logit.
+struct Weigh {
+    const uint2 *power;
+    float high, rate, rate_low;  // log2(e) / temperature = rate + rate_low
+    // of distance + distance_low >= 0; beyond 2^-43, overflow and NaN are nothing
+    __device__ inline uint64_t at(float distance, float distance_low) const {
+        const float y = distance * rate;
+        if (!(y < 43.0f)) return 0;
+        const float y_low = fmaf(distance, rate, -y) + fmaf(distance, rate_low, distance_low * rate);
+        const float shifted = fmaf(y, 256.0f, 12582912.0f);  // 1.5 x 2^23: the nearest whole number of 1/256
+        const uint32_t k = __float_as_uint(shifted) - 0x4b400000u;
+        const float rest = fmaf(shifted - 12582912.0f, -1.0f / 256.0f, y) + y_low;
+        const float q = rest * -0.693147180559945309f;
+        const float more = q * fmaf(q, fmaf(q, 0.16666667f, 0.5f), 1.0f);  // 2^-rest - 1; q^4 / 24 < 2^-42
+        const uint2 base = power[k & 255u];
+        const uint32_t add = __float_as_uint(fmaf(__uint_as_float(base.y), more, 12582912.0f)) - 0x4b400000u;
+        const uint32_t n = k >> 8;
+        return (((uint64_t)(base.x + add) << 11) + ((1ull << n) >> 1)) >> n;
+    }
+    __device__ inline uint64_t of(float x) const {
+        if (x == high) return kOne;
+        const float d = high - x;
+        const float back = high - d;          // d + low = high - x exactly
+        const float low = (high - (d + back)) + (back - x);
+        return at(d, low);
+    }
+};
+// The bin of a distance, before it is cut off to a whole number.
+__device__ inline float place_of(float x, float high, float to_bin, float last) {
+    return x == high ? 0.0f : fminf((high - x) * to_bin, last);  // NaN (0 x infinity) is the last bin
+}
+__device__ inline uint32_t whole(float v) { return __float_as_uint(__fadd_rd(v, 8388608.0f)) & 0x7fffffu; }
+
+// The sum of a value over the threads of the blocks in front of this one, and over those in front of this thread in its own;
+// `all` is the sum over the cluster.  `slot` separates what is exchanged between two cluster barriers; the caller's
+// barrier comes between tell_parts and sum_parts.
+__device__ inline uint64_t tell_parts(cg::cluster_group &cluster, SampleShared &sh, uint32_t slot, uint64_t value) {
+    uint64_t before;
+    const uint64_t sum = block_scan(value, sh.warp_values, before);
+    if (threadIdx.x < cluster.num_blocks()) cluster.map_shared_rank(&sh, threadIdx.x)->parts[slot][cluster.block_rank()] = sum;
+    return before;
+}
+__device__ inline uint64_t sum_parts(cg::cluster_group &cluster, const SampleShared &sh, uint32_t slot, uint64_t &all) {
+    uint64_t before = 0;
+    all = 0;
+    for (uint32_t r = 0; r < cluster.num_blocks(); ++r) {
+        if (r < cluster.block_rank()) before += sh.parts[slot][r];
+        all += sh.parts[slot][r];
+    }
+    return before;
+}
+// This thread's bin over the whole cluster: block r of n has bins [r, r + 1) x bins / n.
+__device__ inline uint32_t my_bin(cg::cluster_group &cluster, uint32_t bins) {
+    const uint32_t each = bins / cluster.num_blocks();
+    return threadIdx.x < each ? cluster.block_rank() * each + threadIdx.x : 0xffffffffu;
+}
+__device__ inline uint32_t count_of(cg::cluster_group &cluster, SampleShared &sh, uint32_t bin) {
+    uint32_t sum = 0;
+    if (bin != 0xffffffffu)
+        for (uint32_t r = 0; r < cluster.num_blocks(); ++r) sum += cluster.map_shared_rank(&sh, r)->count[bin];
+    return sum;
+}
+__device__ inline uint64_t mass_of(cg::cluster_group &cluster, SampleShared &sh, uint32_t bin) {
+    uint64_t sum = 0;
+    if (bin != 0xffffffffu)
+        for (uint32_t r = 0; r < cluster.num_blocks(); ++r) sum += cluster.map_shared_rank(&sh, r)->mass[bin];
+    return sum;
+}
+__device__ inline uint64_t reach_of(float share, uint64_t total) {
+    const double reach = ceil((double)fmaxf(share, 0.0f) * (double)total);
+    return reach < 1.0 ? 1ull : (uint64_t)reach;
+}
+
+// The composite of the last element that stays, over the whole cluster, in every case.  By count: the `wanted`-th element
+// of those at or above `floor`.  By mass: the first at which the running weight reaches `wanted`.
 template <bool MASS, typename T>
-__device__ uint64_t find_cut(cg::cluster_group &cluster, SampleShared &sh, const Slice<T> &slice, const Weigh &weigh,
-                             float low, uint64_t floor, uint64_t wanted) {
+__device__ __noinline__ uint64_t find_cut(cg::cluster_group &cluster, SampleShared &sh, const Slice<T> &slice, const Weigh &weigh,
+                             float to_bin, uint32_t bins, uint64_t floor, uint64_t wanted) {
     const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
-    const uint32_t per_block = kBins / blocks;
     bool by_distance = true;
-    const float to_bin = (float)(kBins - 1) / fmaxf(weigh.high - low, 1e-30f);
     uint64_t span_low = floor, span_high = ~0ull;  // composites still in question, and how they are cut into bins
     uint32_t shift = 0;
     uint64_t before = 0;                           // count or mass above the span
     auto bin_of = [&](float x, uint64_t c) -> uint32_t {
-        if (by_distance) return x == weigh.high ? 0u : (uint32_t)fminf((weigh.high - x) * to_bin, (float)(kBins - 1));
-        return (uint32_t)((span_high - c) >> shift);
+        return by_distance ? whole(place_of(x, weigh.high, to_bin, (float)(bins - 1))) : (uint32_t)((span_high - c) >> shift);
     };
+    auto in_span = [&](uint64_t c) { return c >= span_low && c <= span_high; };
     for (;;) {
         for (uint32_t b = threadIdx.x; b < kBins; b += kSampleThreads) {
             sh.count[b] = 0;
@@ -156,120 +285,56 @@ __device__ uint64_t find_cut(cg::cluster_group &cluster, SampleShared &sh, const
         }
         if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
-        for (uint32_t i = threadIdx.x; i < slice.size; i += kSampleThreads) {
-            const float x = slice.at(i);
+        slice.each([&](float x, uint32_t i) {
             const uint64_t c = composite(x, slice.begin + i);
-            if (c < span_low || c > span_high) continue;
+            if (!in_span(c)) return;
             const uint32_t b = bin_of(x, c);
             atomicAdd(&sh.count[b], 1u);
-            if (MASS) {
-                const uint64_t w = Weigh::units(weigh.real(x));
-                if (w != 0) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[b]), (unsigned long long)w);
-            }
-        }
+            if (MASS) atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[b]), (unsigned long long)weigh.of(x));
+        });
         cluster.sync();
-        // every block adds up its share of the bins over the cluster, tells the others the sum, ...
-        uint64_t my_count = 0, my_mass = 0;
-        if (threadIdx.x < per_block) {
-            const uint32_t b = rank * per_block + threadIdx.x;
-            for (uint32_t r = 0; r < blocks; ++r) {
-                const SampleShared *other = cluster.map_shared_rank(&sh, r);
-                my_count += other->count[b];
-                if (MASS) my_mass += other->mass[b];
-            }
-        }
-        if (blocks == 1) {  // 2048 bins, 1024 threads: two neighbours each
-            my_count = my_mass = 0;
-        }
-        const uint32_t bins_each = per_block > kSampleThreads ? per_block / kSampleThreads : 1;
-        const uint32_t bin0 = rank * per_block + threadIdx.x * bins_each;
-        uint64_t each_count[2] = {my_count, 0}, each_mass[2] = {my_mass, 0};
-        if (bins_each == 2) {
-            for (uint32_t e = 0; e < 2; ++e) {
-                each_count[e] = sh.count[bin0 + e];
-                if (MASS) each_mass[e] = sh.mass[bin0 + e];
-            }
-            my_count = each_count[0] + each_count[1];
-            my_mass = each_mass[0] + each_mass[1];
-        }
-        const uint64_t sum_count = block_sum(my_count, sh.warp_values);
-        const uint64_t sum_mass = MASS ? block_sum(my_mass, sh.warp_values) : 0;
-        if (threadIdx.x < blocks) {
-            SampleShared *other = cluster.map_shared_rank(&sh, threadIdx.x);
-            other->part_count[rank] = sum_count;
-            other->part_mass[rank] = sum_mass;
-        }
-        cluster.sync();
-        // ... and the one whose share holds the border finds its bin
-        uint64_t parts_before = before;
-        for (uint32_t r = 0; r < rank; ++r) parts_before += MASS ? sh.part_mass[r] : sh.part_count[r];
-        uint32_t owner = blocks;
-        {
-            uint64_t sum = before;
-            for (uint32_t r = 0; r < blocks; ++r) {
-                sum += MASS ? sh.part_mass[r] : sh.part_count[r];
-                if (owner == blocks && sum >= wanted) owner = r;
-            }
-        }
-        if (owner == blocks) {  // fewer than wanted: everything stays
+        const uint32_t bin = my_bin(cluster, bins), number = count_of(cluster, sh, bin);
+        const uint64_t own = MASS ? mass_of(cluster, sh, bin) : number;
+        uint64_t running = tell_parts(cluster, sh, 0, own), all;
+        cluster.sync();  // the bins have been read everywhere: the list may take their place
+        running += before + sum_parts(cluster, sh, 0, all);
+        if (before + all < wanted) {  // everything stays
             cluster.sync();
             return floor;
         }
-        if (owner == rank) {
-            // exclusive running value of this thread's bins
-            uint64_t inclusive = MASS ? my_mass : my_count;
-            const uint64_t own = inclusive;
-            const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const uint64_t y = __shfl_up_sync(0xffffffffu, inclusive, d);
-                if (lane >= (uint32_t)d) inclusive += y;
-            }
-            if (lane == 31) sh.warp_values[warp] = inclusive;
-            __syncthreads();
-            uint64_t exclusive = parts_before + inclusive - own;
-            for (uint32_t w = 0; w < warp; ++w) exclusive += sh.warp_values[w];
-            for (uint32_t e = 0; e < bins_each; ++e) {
-                const uint64_t value = MASS ? each_mass[e] : each_count[e];
-                if (value != 0 && exclusive < wanted && exclusive + value >= wanted) {
-                    for (uint32_t r = 0; r < blocks; ++r) {
-                        SampleShared *other = cluster.map_shared_rank(&sh, r);
-                        other->border = bin0 + e;
-                        other->border_count = (uint32_t)each_count[e];
-                        other->before_mass = exclusive;
-                    }
-                }
-                exclusive += value;
+        if (own != 0 && running < wanted && running + own >= wanted) {
+            for (uint32_t r = 0; r < blocks; ++r) {
+                SampleShared *other = cluster.map_shared_rank(&sh, r);
+                other->low_bin = bin;
+                other->found_count = number;
+                other->found_before = running;
             }
         }
         cluster.sync();
-        const uint32_t border = sh.border, border_count = sh.border_count;
-        before = sh.before_mass;
+        const uint32_t border = sh.low_bin, border_count = sh.found_count;
+        before = sh.found_before;
         if (border_count <= kListed) {
-            // gather the bin in the first block and rank it
+            // gather the bin in the first block and rank it there
             SampleShared *leader = cluster.map_shared_rank(&sh, 0);
-            for (uint32_t i = threadIdx.x; i < slice.size; i += kSampleThreads) {
-                const float x = slice.at(i);
+            slice.each([&](float x, uint32_t i) {
                 const uint64_t c = composite(x, slice.begin + i);
-                if (c < span_low || c > span_high || bin_of(x, c) != border) continue;
-                leader->list[atomicAdd(&leader->listed, 1u)] = c;
-            }
+                if (in_span(c) && bin_of(x, c) == border) leader->list[atomicAdd(&leader->listed, 1u)] = c;
+            });
             cluster.sync();
             if (rank == 0) {
                 const uint32_t n = sh.listed;
                 if (MASS) {
-                    for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads)
-                        sh.list_weight[i] = Weigh::units(weigh.real(logit_of(sh.list[i])));
+                    for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) sh.sums[i] = weigh.of(logit_of(sh.list[i]));
                     __syncthreads();
                 }
                 for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) {
                     const uint64_t c = sh.list[i];
                     uint64_t above = before;
                     for (uint32_t j = 0; j < n; ++j) {
-                        if (sh.list[j] > c) above += MASS ? sh.list_weight[j] : 1u;
+                        if (sh.list[j] > c) above += MASS ? sh.sums[j] : 1u;
                     }
-                    const uint64_t own = MASS ? sh.list_weight[i] : 1u;
-                    if (above < wanted && above + own >= wanted) {
+                    const uint64_t mine = MASS ? sh.sums[i] : 1u;
+                    if (above < wanted && above + mine >= wanted) {
                         for (uint32_t r = 0; r < blocks; ++r) cluster.map_shared_rank(&sh, r)->cut = c;
                     }
                 }
@@ -279,13 +344,12 @@ __device__ uint64_t find_cut(cg::cluster_group &cluster, SampleShared &sh, const
         }
         // too many for that: what span do they cover?
         uint64_t c_low = ~0ull, c_high = 0;
-        for (uint32_t i = threadIdx.x; i < slice.size; i += kSampleThreads) {
-            const float x = slice.at(i);
+        slice.each([&](float x, uint32_t i) {
             const uint64_t c = composite(x, slice.begin + i);
-            if (c < span_low || c > span_high || bin_of(x, c) != border) continue;
+            if (!in_span(c) || bin_of(x, c) != border) return;
             c_low = c < c_low ? c : c_low;
             c_high = c > c_high ? c : c_high;
-        }
+        });
         c_low = ~block_max(~c_low, sh.warp_values);
         c_high = block_max(c_high, sh.warp_values);
         if (threadIdx.x < blocks) {
@@ -301,138 +365,451 @@ __device__ uint64_t find_cut(cg::cluster_group &cluster, SampleShared &sh, const
             span_high = sh.span_high[r] > span_high ? sh.span_high[r] : span_high;
         }
         by_distance = false;
-        const uint32_t bits = 64 - __clzll((long long)(span_high - span_low));
-        shift = bits > 11 ? bits - 11 : 0;  // bins 0 .. (span >> shift) < 2048
+        const uint32_t bits = 64 - __clzll((long long)(span_high - span_low)), room = 31 - __clz(bins);
+        shift = bits > room ? bits - room : 0;  // bins 0 .. (span >> shift) < bins
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kSampleThreads, 1)
-sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size, uint32_t kept_on_chip) {
+// Largest first (or smallest, for UP), over the next power of two of n; the caller has filled the rest with the least.
+template <bool UP, typename V>
+__device__ void block_sort(V *values, uint32_t n) {
+    uint32_t size = 32;
+    while (size < n) size *= 2;
+    for (uint32_t k = 2; k <= size; k *= 2) {
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+            for (uint32_t pair = threadIdx.x; pair < size / 2; pair += kSampleThreads) {
+                const uint32_t i = 2 * pair - (pair & (j - 1)), other = i + j;
+                const V x = values[i], y = values[other];
+                if ((x > y) == (((i & k) == 0) != UP ? false : true)) {
+                    values[i] = y;
+                    values[other] = x;
+                }
+            }
+            __syncthreads();
+        }
+    }
+}
+
+__device__ inline uint64_t target_of(float uniform, uint64_t total) {
+    const double aim = uniform > 0.0f ? floor((double)uniform * (double)total) : 0.0;
+    const uint64_t target = aim < (double)total ? (uint64_t)aim : total - 1;
+    return target < total ? target : total - 1;
+}
+
+// All that matter are in this block's list: cut them, draw, and answer.  `mass` is the sum that top-p is a share of, or 0
+// where it is the sum of the first k.
+__device__ __noinline__ void finish_list(const SampleArgs &p, uint32_t row, SampleShared &sh, const Weigh &weigh, uint32_t k,
+                                         float share, uint64_t mass, uint64_t least) {
+    const uint32_t n = sh.listed;
+    uint32_t size = 32;
+    while (size < n) size *= 2;
+    for (uint32_t i = n + threadIdx.x; i < size; i += kSampleThreads) sh.list[i] = 0;
+    __syncthreads();
+    if (n > kSampleThreads) block_sort<false>(sh.list, n);
+    const uint32_t first = k != 0 && k < n ? k : n;
+    const float uniform = p.uniform[row];
+    if (n <= kSampleThreads) {
+        // an element per thread, ranked against all others: fewer steps than sorting twice
+        const uint32_t i = threadIdx.x;
+        const uint64_t own = i < n ? sh.list[i] : 0, weight = i < n ? weigh.of(logit_of(own)) : 0;
+        if (i < n) sh.sums[i] = weight;
+        __syncthreads();
+        uint32_t place = 0;
+        uint64_t above = 0;
+        if (i < n) {
+#pragma unroll 4
+            for (uint32_t j = 0; j < n; ++j) {
+                if (sh.list[j] > own) {
+                    ++place;
+                    above += sh.sums[j];
+                }
+            }
+        }
+        bool stays = i < n && place < first;
+        const uint64_t whole_sum = mass != 0 || !(share < 1.0f) ? mass : block_sum(stays ? weight : 0, sh.warp_values);
+        if (share < 1.0f) stays = stays && above < reach_of(share, whole_sum);
+        stays = stays && weight >= least;
+        const uint64_t total = block_sum(stays ? weight : 0, sh.warp_values);
+        __syncthreads();
+        if (i < n) sh.sums[i] = stays ? weight : 0;
+        __syncthreads();
+        if (!stays) return;
+        uint64_t running = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < n; ++j)
+            if ((uint32_t)sh.list[j] > (uint32_t)own) running += sh.sums[j];  // a smaller index: its complement is larger
+        const uint64_t target = target_of(uniform, total);
+        if (running <= target && running + weight > target) {
+            p.tokens[row] = index_of(own);
+            if (p.probabilities != nullptr) p.probabilities[row] = (float)((double)weight / (double)total);
+        }
+        return;
+    }
+    // in order: running weights, four neighbours per thread
+    uint64_t weight[4], own = 0, running;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        const uint32_t i = 4 * threadIdx.x + e;
+        weight[e] = i < n ? weigh.of(logit_of(sh.list[i])) : 0;
+        own += weight[e];
+    }
+    block_scan(own, sh.warp_values, running);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        running += weight[e];
+        sh.sums[4 * threadIdx.x + e] = running;
+    }
+    __syncthreads();
+    const uint64_t wanted = share < 1.0f ? reach_of(share, mass != 0 ? mass : sh.sums[first - 1]) : ~0ull;
+    uint32_t stay = 0;  // how many stay: a prefix
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        const uint32_t i = 4 * threadIdx.x + e;
+        if (i < first && sh.sums[i] - weight[e] < wanted && weight[e] >= least) ++stay;
+    }
+    const uint32_t m = (uint32_t)block_sum(stay, sh.warp_values);
+    const uint64_t total = sh.sums[m - 1];
+    // by index: (index, place in the order) as one number
+    uint32_t *const by_index = sh.count;
+    size = 32;
+    while (size < m) size *= 2;
+    for (uint32_t i = threadIdx.x; i < size; i += kSampleThreads)
+        by_index[i] = i < m ? index_of(sh.list[i]) << 11 | i : 0xffffffffu;
+    __syncthreads();
+    block_sort<true>(by_index, m);
+    own = 0;
+    uint32_t place[4];
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        const uint32_t i = 4 * threadIdx.x + e;
+        place[e] = i < m ? by_index[i] & (kListed - 1) : 0;
+        weight[e] = i < m ? sh.sums[place[e]] - (place[e] > 0 ? sh.sums[place[e] - 1] : 0) : 0;
+        own += weight[e];
+    }
+    block_scan(own, sh.warp_values, running);
+    const uint64_t target = target_of(uniform, total);
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) {
+        if (running <= target && running + weight[e] > target) {
+            p.tokens[row] = index_of(sh.list[place[e]]);
+            if (p.probabilities != nullptr) p.probabilities[row] = (float)((double)weight[e] / (double)total);
+        }
+        running += weight[e];
+    }
+}
+
+template <typename T, bool ON_CHIP>
+__global__ void __launch_bounds__(kSampleThreads, ON_CHIP ? 1 : 2)
+sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ __align__(16) uint8_t sample_smem[];
     SampleShared &sh = *reinterpret_cast<SampleShared *>(sample_smem);
     uint64_t *const tiles = reinterpret_cast<uint64_t *>(sample_smem + sizeof(SampleShared));
-    uint8_t *const held = reinterpret_cast<uint8_t *>(tiles + ceil_div(slice_size, kTile));
     const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t row = blockIdx.x / blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
-    const T *const logits = static_cast<const T *>(p.logits) + (size_t)row * p.ld;
     Slice<T> slice;
     slice.begin = min(rank * slice_size, p.vocab);
     slice.size = min(slice_size, p.vocab - slice.begin);
-    slice.data = logits + slice.begin;
+    slice.data = static_cast<const T *>(p.logits) + (size_t)row * p.ld + slice.begin;
+    const uint32_t skew = (uint32_t)(reinterpret_cast<uintptr_t>(slice.data) & 15u);
+    slice.split(skew);
+    cg::cluster_group::arrival_token running_token = cluster.barrier_arrive();
 
-    // ---- load ----
-    uint64_t best = 0;
-    float low = INFINITY;
-    auto look = [&](float raw, uint32_t i) {
-        const float x = tidy(raw);
-        const uint64_t c = composite(x, slice.begin + i);
-        best = c > best ? c : best;
+    // ---- load: extremes on the way ----
+    float high = -INFINITY, low = INFINITY;
+    auto look = [&](float x, uint32_t) {
+        high = fmaxf(high, x);
         if (x > -INFINITY) low = fminf(low, x);
     };
-    if (kept_on_chip) {
-        // the copy starts at the same place within 16 bytes as the original, so whole 16-byte words move
-        const uint32_t skew = (uint32_t)(reinterpret_cast<uintptr_t>(slice.data) & 15u);
-        uint8_t *const place = held + ((16u - (uint32_t)(reinterpret_cast<uintptr_t>(held) & 15u)) & 15u) + skew;
-        T *const copy = reinterpret_cast<T *>(place);
-        constexpr uint32_t kWord = 16 / sizeof(T);
-        const uint32_t head = min(slice.size, skew == 0 ? 0u : (16u - skew) / (uint32_t)sizeof(T));
-        const uint32_t words = (slice.size - head) / kWord, tail = head + words * kWord;
-        if (threadIdx.x < head) {
-            copy[threadIdx.x] = slice.data[threadIdx.x];
-            look(as_float(slice.data[threadIdx.x]), threadIdx.x);
-        }
-        const uint4 *from = reinterpret_cast<const uint4 *>(slice.data + head);
-        uint4 *to = reinterpret_cast<uint4 *>(copy + head);
-#pragma unroll 4
-        for (uint32_t w = threadIdx.x; w < words; w += kSampleThreads) {
-            const uint4 word = __ldcs(from + w);
-            to[w] = word;
-            const T *x = reinterpret_cast<const T *>(&word);
+    if (ON_CHIP) {
+        // the copy starts at the same place within 16 bytes as the original, so whole words move
+        uint8_t *held = reinterpret_cast<uint8_t *>(tiles + slice.tiles() + 2);
+        held += ((16u - (uint32_t)(reinterpret_cast<uintptr_t>(held) & 15u)) & 15u) + skew;
+        T *const copy = reinterpret_cast<T *>(held);
+        const uint4 *const from = reinterpret_cast<const uint4 *>(slice.data + slice.head);
+        uint4 *const to = reinterpret_cast<uint4 *>(copy + slice.head);
+        for (uint32_t w0 = threadIdx.x; w0 < slice.words; w0 += 8 * kSampleThreads) {
+            uint4 word[8];
 #pragma unroll
-            for (uint32_t j = 0; j < kWord; ++j) look(as_float(x[j]), head + w * kWord + j);
+            for (uint32_t u = 0; u < 8; ++u)
+                if (w0 + u * kSampleThreads < slice.words) word[u] = __ldcs(from + w0 + u * kSampleThreads);
+#pragma unroll
+            for (uint32_t u = 0; u < 8; ++u) {
+                if (w0 + u * kSampleThreads < slice.words) {
+                    to[w0 + u * kSampleThreads] = word[u];
+                    const T *x = reinterpret_cast<const T *>(&word[u]);
+#pragma unroll
+                    for (uint32_t j = 0; j < Slice<T>::kWord; ++j) look(tidy(as_float(x[j])), 0);
+                }
+            }
         }
-        if (tail + threadIdx.x < slice.size) {
-            copy[tail + threadIdx.x] = slice.data[tail + threadIdx.x];
-            look(as_float(slice.data[tail + threadIdx.x]), tail + threadIdx.x);
+        if (threadIdx.x < slice.head + slice.tail) {
+            const uint32_t i = threadIdx.x < slice.head ? threadIdx.x : slice.size - slice.tail + threadIdx.x - slice.head;
+            copy[i] = slice.data[i];
+            look(slice.at(i), 0);
         }
         slice.data = copy;
     } else {
-        for (uint32_t i = threadIdx.x; i < slice.size; i += kSampleThreads) look(as_float(slice.data[i]), i);
+        slice.each(look);
     }
-    best = block_max(best, sh.warp_values);
-    low = block_min(low, sh.warp_low);
-    cluster.sync();  // every block of the cluster runs: its shared memory may be written
-    if (threadIdx.x < blocks) {
-        SampleShared *other = cluster.map_shared_rank(&sh, threadIdx.x);
-        other->high[rank] = best;
-        other->low[rank] = low;
+    if (threadIdx.x < 256) sh.power[threadIdx.x] = kPowers.entry[threadIdx.x];
+    for (uint32_t b = threadIdx.x; b < kBins; b += kSampleThreads) sh.count[b] = 0;
+    if (threadIdx.x == 0) {
+        sh.listed = 0;
+        sh.first = 0xffffffffu;
+    }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+        low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
+    }
+    if (lane == 0) {
+        sh.warp_high[warp] = high;
+        sh.warp_low[warp] = low;
+    }
+    __syncthreads();
+    cluster.barrier_wait(static_cast<cg::cluster_group::arrival_token &&>(running_token));  // every block of the cluster runs
+    if (warp == 0) {
+        high = sh.warp_high[lane & (kSampleWarps - 1)];
+        low = sh.warp_low[lane & (kSampleWarps - 1)];
+#pragma unroll
+        for (int d = kSampleWarps / 2; d > 0; d >>= 1) {
+            high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+            low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
+        }
+        if (lane < blocks) {
+            SampleShared *other = cluster.map_shared_rank(&sh, lane);
+            other->high[rank] = high;
+            other->low[rank] = low;
+        }
     }
     cluster.sync();
-    for (uint32_t r = 0; r < blocks; ++r) {
-        best = sh.high[r] > best ? sh.high[r] : best;
+    high = sh.high[0];
+    low = sh.low[0];
+    for (uint32_t r = 1; r < blocks; ++r) {
+        high = fmaxf(high, sh.high[r]);
         low = fminf(low, sh.low[r]);
     }
-    Weigh weigh;
-    weigh.high = logit_of(best);
     const float temperature = p.temperature != nullptr ? p.temperature[row] : 1.0f;
-    if (weigh.high == -INFINITY || !(temperature > 0.0f)) {
+    if (high == -INFINITY) {
         if (rank == 0 && threadIdx.x == 0) {
-            const bool none = weigh.high == -INFINITY;
-            p.tokens[row] = none ? 0xffffffffu : index_of(best);
-            if (p.probabilities != nullptr) p.probabilities[row] = none ? 0.0f : 1.0f;
+            p.tokens[row] = 0xffffffffu;
+            if (p.probabilities != nullptr) p.probabilities[row] = 0.0f;
         }
-        return;  // the same decision in every block of the cluster, and nobody's shared memory is read any more
+        return;
     }
-    weigh.over = 1.0 / (double)temperature;
-
-    // ---- the cuts ----
-    uint64_t cut = 0;
-    const uint32_t k = p.top_k != nullptr ? p.top_k[row] : 0;
-    if (k != 0 && k < p.vocab) cut = find_cut<false>(cluster, sh, slice, weigh, low, 0ull, (uint64_t)k);
-    const float share = p.top_p != nullptr ? p.top_p[row] : 1.0f;
-    if (share < 1.0f) {
-        uint64_t mine = 0;
-        for (uint32_t i = threadIdx.x; i < slice.size; i += kSampleThreads) {
-            const float x = slice.at(i);
-            if (composite(x, slice.begin + i) >= cut) mine += Weigh::units(weigh.real(x));
-        }
-        mine = block_sum(mine, sh.warp_values);
-        if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->total[rank] = mine;
+    if (!(temperature > 0.0f)) {
+        uint32_t first = 0xffffffffu;
+        slice.each([&](float x, uint32_t i) {
+            if (x == high) first = min(first, slice.begin + i);
+        });
+        first = __reduce_min_sync(0xffffffffu, first);
+        if (lane == 0 && first != 0xffffffffu) atomicMin(&cluster.map_shared_rank(&sh, 0)->first, first);
         cluster.sync();
-        uint64_t total = 0;
-        for (uint32_t r = 0; r < blocks; ++r) total += sh.total[r];
-        const double wanted = ceil((double)fmaxf(share, 0.0f) * (double)total);
-        cut = find_cut<true>(cluster, sh, slice, weigh, low, cut, wanted < 1.0 ? 1ull : (uint64_t)wanted);
+        if (rank == 0 && threadIdx.x == 0) {
+            p.tokens[row] = sh.first;
+            if (p.probabilities != nullptr) p.probabilities[row] = 1.0f;
+        }
+        return;
     }
-    double least = p.min_p != nullptr ? (double)p.min_p[row] : 0.0;
-    if (least > 1.0) least = 1.0;
-    auto kept_units = [&](uint32_t i) -> uint64_t {
-        const float x = slice.at(i);
-        if (composite(x, slice.begin + i) < cut) return 0;
-        const double w = weigh.real(x);
-        return w < least ? 0ull : Weigh::units(w);
-    };
+    Weigh weigh;
+    weigh.power = sh.power;
+    weigh.high = high;
+    const double rate = 1.4426950408889634074 / (double)temperature;
+    weigh.rate = (float)rate;
+    weigh.rate_low = weigh.rate < 3.0e38f ? (float)(rate - (double)weigh.rate) : 0.0f;
+    const uint32_t bins = min(kBins, blocks * kSampleThreads);
+    const float last_bin = (float)(bins - 1), to_bin = last_bin / fmaxf(high - low, 1e-30f);
+    const uint32_t k = p.top_k != nullptr && p.top_k[row] < p.vocab ? p.top_k[row] : 0;
+    const float share = p.top_p != nullptr ? p.top_p[row] : 1.0f;
+    const float floor_p = p.min_p != nullptr ? p.min_p[row] : 0.0f;
+    // the least weight that stays, in units (a NaN is none)
+    const uint64_t least = floor_p > 0.0f ? (uint64_t)ceil((double)fminf(floor_p, 1.0f) * (double)kOne) : 0;
 
-    // ---- the token ----
-    const uint32_t tile_count = ceil_div(slice.size, kTile);
-    for (uint32_t tile = warp; tile < tile_count; tile += kSampleWarps) {
+    uint64_t cut = 0;
+    if (k != 0 || share < 1.0f) {
+        // ---- counts ----
+        const bool add = k == 0;  // top-p alone is a share of everything
+        uint64_t mine = 0;
+        slice.each([&](float x, uint32_t) {
+            atomicAdd(&sh.count[whole(place_of(x, high, to_bin, last_bin))], 1u);
+            if (add) mine += weigh.of(x);
+        });
+        if (add) {
+            mine = block_sum(mine, sh.warp_values);
+            if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->total[rank] = mine;
+        }
+        if (threadIdx.x == 0) {
+            sh.low_bin = sh.high_bin = bins - 1;
+            sh.found_count = sh.fine_count = 0;  // elements down to the end of the bracket, or in its bin; 0: nobody found it
+        }
+        cluster.sync();
+        uint64_t everything = 0, wanted = k;
+        if (add) {
+            for (uint32_t r = 0; r < blocks; ++r) everything += sh.total[r];
+            wanted = reach_of(share, everything);
+        }
+        // By weight a bin of n elements holds between n times the weight at its far edge and n times that at its near one
+        // (the edges moved out by the rounding of a place: two units in the last of 2048).  [low_bin, high_bin] is where
+        // the border may lie; by count both are its bin.
+        const uint32_t bin = my_bin(cluster, bins), number = count_of(cluster, sh, bin);
+        uint64_t far = number, near = number;
+        if (add) {
+            const float b = (float)bin, width = 1.0f / to_bin;
+            uint64_t least_of = b < last_bin ? weigh.at((b + 1.001f) * width, 0.0f) : 0;
+            least_of -= least_of > 0 ? (least_of >> 28) + 1 : 0;  // and by a weight's own error
+            uint64_t most_of = b > 0.0f ? weigh.at((b - 0.001f) * width, 0.0f) : kOne;
+            far = number * least_of;
+            near = number * (most_of + (most_of >> 28) + 1);
+        }
+        uint64_t far_before = tell_parts(cluster, sh, 0, far), near_before = 0, number_before = 0, all_of;
+        if (add) {
+            near_before = tell_parts(cluster, sh, 1, near);
+            number_before = tell_parts(cluster, sh, 2, number);
+        }
+        cluster.sync();  // the bins have been read everywhere
+        far_before += sum_parts(cluster, sh, 0, all_of);
+        if (add) {
+            near_before += sum_parts(cluster, sh, 1, all_of);
+            number_before += sum_parts(cluster, sh, 2, all_of);
+        } else {
+            near_before = number_before = far_before;
+        }
+        const bool is_low = near_before < wanted && near_before + near >= wanted;
+        const bool is_high = far_before < wanted && far_before + far >= wanted;
+        if (number != 0 && (is_low || is_high)) {
+            for (uint32_t r = 0; r < blocks; ++r) {
+                SampleShared *other = cluster.map_shared_rank(&sh, r);
+                if (is_low) other->low_bin = bin;
+                if (is_high) {
+                    other->high_bin = bin;
+                    other->found_count = (uint32_t)number_before + number;
+                }
+            }
+        }
+        cluster.sync();
+        const uint32_t low_bin = sh.low_bin, high_bin = sh.high_bin, down_to = sh.found_count;
+        if (down_to != 0 && down_to <= kListed) {
+            // ---- few stay ----
+            SampleShared *leader = cluster.map_shared_rank(&sh, 0);
+            const float end = (float)(high_bin + 1);
+            slice.each([&](float x, uint32_t i) {
+                if (place_of(x, high, to_bin, last_bin) < end) leader->list[atomicAdd(&leader->listed, 1u)] = composite(x, slice.begin + i);
+            });
+            cluster.sync();
+            if (rank == 0) finish_list(p, row, sh, weigh, k, share, everything, least);
+            return;
+        }
+        if (add) {
+            // ---- many stay: the bracket by exact weights ----
+            for (uint32_t b = threadIdx.x; b < bins; b += kSampleThreads) {
+                sh.count[b] = 0;
+                sh.mass[b] = 0;
+            }
+            __syncthreads();
+            const float first = (float)low_bin, end = (float)(high_bin + 1), finer = (float)bins / (end - first);
+            uint64_t above = 0;
+            auto fine_bin = [&](float v) { return whole(fminf((v - first) * finer, last_bin)); };
+            slice.each([&](float x, uint32_t) {
+                const float v = place_of(x, high, to_bin, last_bin);
+                if (v >= end) return;
+                const uint64_t w = weigh.of(x);
+                if (v < first) {
+                    above += w;
+                } else {
+                    const uint32_t b = fine_bin(v);
+                    atomicAdd(&sh.count[b], 1u);
+                    atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[b]), (unsigned long long)w);
+                }
+            });
+            tell_parts(cluster, sh, 1, above);
+            cluster.sync();
+            const uint32_t fine_number = count_of(cluster, sh, bin);
+            const uint64_t own = mass_of(cluster, sh, bin);
+            uint64_t running = tell_parts(cluster, sh, 0, own), all_above;
+            sum_parts(cluster, sh, 1, all_above);
+            cluster.sync();  // the bins have been read everywhere: the list may take their place
+            running += all_above + sum_parts(cluster, sh, 0, all_of);
+            if (own != 0 && running < wanted && running + own >= wanted) {
+                for (uint32_t r = 0; r < blocks; ++r) {
+                    SampleShared *other = cluster.map_shared_rank(&sh, r);
+                    other->fine_bin = bin;
+                    other->fine_count = fine_number;
+                    other->found_before = running;
+                }
+            }
+            cluster.sync();
+            const uint32_t border = sh.fine_bin, border_count = sh.fine_count;
+            const uint64_t before = sh.found_before;
+            if (border_count != 0 && border_count <= kListed) {
+                SampleShared *leader = cluster.map_shared_rank(&sh, 0);
+                slice.each([&](float x, uint32_t i) {
+                    const float v = place_of(x, high, to_bin, last_bin);
+                    if (v >= first && v < end && fine_bin(v) == border)
+                        leader->list[atomicAdd(&leader->listed, 1u)] = composite(x, slice.begin + i);
+                });
+                cluster.sync();
+                if (rank == 0) {
+                    const uint32_t n = sh.listed;
+                    for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) sh.sums[i] = weigh.of(logit_of(sh.list[i]));
+                    __syncthreads();
+                    for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) {
+                        const uint64_t c = sh.list[i];
+                        uint64_t over = before;
+#pragma unroll 4
+                        for (uint32_t j = 0; j < n; ++j)
+                            if (sh.list[j] > c) over += sh.sums[j];
+                        if (over < wanted && over + sh.sums[i] >= wanted)
+                            for (uint32_t r = 0; r < blocks; ++r) cluster.map_shared_rank(&sh, r)->cut = c;
+                    }
+                }
+                cluster.sync();
+                cut = sh.cut;
+            } else {
+                cut = find_cut<true>(cluster, sh, slice, weigh, to_bin, bins, 0ull, wanted);
+            }
+        } else {
+            cut = find_cut<false>(cluster, sh, slice, weigh, to_bin, bins, 0ull, wanted);
+            if (share < 1.0f) {
+                mine = 0;
+                slice.each([&](float x, uint32_t i) {
+                    if (composite(x, slice.begin + i) >= cut) mine += weigh.of(x);
+                });
+                mine = block_sum(mine, sh.warp_values);
+                if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->total[rank] = mine;
+                cluster.sync();
+                for (uint32_t r = 0; r < blocks; ++r) everything += sh.total[r];
+                cut = find_cut<true>(cluster, sh, slice, weigh, to_bin, bins, cut, reach_of(share, everything));
+            }
+        }
+    }
+
+    // ---- the token: sums per tile (the head is one of its own in front, the tail one behind) ----
+    const bool all = cut == 0;
+    auto kept = [&](float x, uint32_t i) -> uint64_t {
+        if (!all && composite(x, slice.begin + i) < cut) return 0;
+        const uint64_t w = weigh.of(x);
+        return w < least ? 0ull : w;
+    };
+    const uint32_t word_tiles = slice.tiles(), tile_count = word_tiles + 2;
+    for (uint32_t t = warp; t < tile_count; t += kSampleWarps) {
         uint64_t sum = 0;
-#pragma unroll
-        for (uint32_t j = 0; j < kTile / 32; ++j) {
-            const uint32_t i = tile * kTile + j * 32 + lane;
-            if (i < slice.size) sum += kept_units(i);
+        if (t == 0) {
+            if (lane < slice.head) sum = kept(slice.at(lane), lane);
+        } else if (t == tile_count - 1) {
+            if (lane < slice.tail) sum = kept(slice.at(slice.size - slice.tail + lane), slice.size - slice.tail + lane);
+        } else {
+            slice.tile(t - 1, [&](float x, uint32_t i) { sum += kept(x, i); });
         }
         sum = warp_sum(sum);
-        if (lane == 0) tiles[tile] = sum;
+        if (lane == 0) tiles[t] = sum;
     }
     __syncthreads();
     uint64_t mine = 0;
-    for (uint32_t tile = threadIdx.x; tile < tile_count; tile += kSampleThreads) mine += tiles[tile];
+    for (uint32_t t = threadIdx.x; t < tile_count; t += kSampleThreads) mine += tiles[t];
     mine = block_sum(mine, sh.warp_values);
-    cluster.sync();  // sh.total of the top-p pass has been read everywhere
+    // (the sums of the top-p passes have been read everywhere: a cluster barrier lies between)
     if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->total[rank] = mine;
     cluster.sync();  // the last look into another block's shared memory is behind this
     uint64_t total = 0, before = 0;
@@ -440,22 +817,14 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size, uint32_
         if (r < rank) before += sh.total[r];
         total += sh.total[r];
     }
-    const float uniform = p.uniform[row];
-    const double aim = uniform > 0.0f ? floor((double)uniform * (double)total) : 0.0;
-    uint64_t target = aim < (double)total ? (uint64_t)aim : total - 1;
-    if (target > total - 1) target = total - 1;
+    const uint64_t target = target_of(p.uniform[row], total);
     if (target < before || target >= before + mine || warp != 0) return;
     // the tile, 32 at a time
     uint64_t running = before;
     uint32_t tile = 0;
     for (uint32_t t0 = 0; t0 < tile_count; t0 += 32) {
         const uint64_t own = t0 + lane < tile_count ? tiles[t0 + lane] : 0;
-        uint64_t inclusive = own;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const uint64_t y = __shfl_up_sync(0xffffffffu, inclusive, d);
-            if (lane >= (uint32_t)d) inclusive += y;
-        }
+        const uint64_t inclusive = warp_inclusive(own);
         const uint32_t passed = __ballot_sync(0xffffffffu, running + inclusive > target);
         if (passed != 0) {
             const int first = __ffs(passed) - 1;
@@ -465,47 +834,41 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size, uint32_
         }
         running += __shfl_sync(0xffffffffu, inclusive, 31);
     }
-    // eight neighbours per lane
-    uint64_t own[kTile / 32], sum = 0;
+    // within it: rows of 32 words, a word per lane (or single values)
+    const bool single = tile == 0 || tile == tile_count - 1;
+    const uint32_t first = tile == 0 ? 0 : single ? slice.size - slice.tail : slice.head + (tile - 1) * kTileWords * Slice<T>::kWord;
+    const uint32_t values = single ? 1 : Slice<T>::kWord, end = tile == 0 ? slice.head : single ? slice.size : slice.head + slice.words * Slice<T>::kWord;
+    for (uint32_t r = 0; r < (single ? 1u : kTileRows4); ++r) {
+        const uint32_t at = first + (r * 32 + lane) * values;
+        uint64_t own[Slice<T>::kWord], sum = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kTile / 32; ++j) {
-        const uint32_t i = tile * kTile + lane * (kTile / 32) + j;
-        own[j] = i < slice.size ? kept_units(i) : 0;
-        sum += own[j];
-    }
-    uint64_t inclusive = sum;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-        const uint64_t y = __shfl_up_sync(0xffffffffu, inclusive, d);
-        if (lane >= (uint32_t)d) inclusive += y;
-    }
-    running += inclusive - sum;
-    if (running <= target && running + sum > target) {
-#pragma unroll
-        for (uint32_t j = 0; j < kTile / 32; ++j) {
-            if (running <= target && running + own[j] > target) {
-                p.tokens[row] = slice.begin + tile * kTile + lane * (kTile / 32) + j;
-                if (p.probabilities != nullptr) p.probabilities[row] = (float)((double)own[j] / (double)total);
-            }
-            running += own[j];
+        for (uint32_t j = 0; j < Slice<T>::kWord; ++j) {
+            own[j] = j < values && at + j < end ? kept(slice.at(at + j), at + j) : 0;
+            sum += own[j];
         }
+        const uint64_t inclusive = warp_inclusive(sum);
+        uint64_t here = running + inclusive - sum;
+        if (here <= target && here + sum > target) {
+#pragma unroll
+            for (uint32_t j = 0; j < Slice<T>::kWord; ++j) {
+                if (here <= target && here + own[j] > target) {
+                    p.tokens[row] = slice.begin + at + j;
+                    if (p.probabilities != nullptr) p.probabilities[row] = (float)((double)own[j] / (double)total);
+                }
+                here += own[j];
+            }
+        }
+        running += __shfl_sync(0xffffffffu, inclusive, 31);
     }
 }
 
-template <typename T>
-cudaError_t launch_sample_of(const SampleArgs &args, cudaStream_t stream) {
-    // blocks per row: at least 4096 logits each, 8 at most
-    uint32_t blocks = 1;
-    while (blocks < kMostBlocks && args.vocab / (2 * blocks) >= 4096) blocks *= 2;
-    const uint32_t slice = ceil_div(args.vocab, blocks);
-    const size_t slice_bytes = (size_t)slice * sizeof(T) + 32;
-    const bool on_chip = slice_bytes <= kSliceBytes;
-    const size_t smem = sizeof(SampleShared) + (size_t)ceil_div(slice, kTile) * 8 + (on_chip ? slice_bytes : 0);
+template <typename T, bool ON_CHIP>
+cudaError_t launch_sample_as(const SampleArgs &args, uint32_t blocks, uint32_t slice, size_t smem, cudaStream_t stream) {
     static bool configured[kMaxDevices] = {};
     const int slot = device_slot();
     if (slot < 0 || !configured[slot]) {
-        cudaError_t status = cudaFuncSetAttribute(sample_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                  (int)(sizeof(SampleShared) + kMostTiles * 8 / kMostBlocks + kSliceBytes));
+        const size_t most = sizeof(SampleShared) + ((1u << 20) / kMostBlocks * 4 / 16 / kTileWords + 3) * 8 + (ON_CHIP ? kSliceBytes : 0);
+        cudaError_t status = cudaFuncSetAttribute(sample_kernel<T, ON_CHIP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (status != cudaSuccess) return status;
         if (slot >= 0) configured[slot] = true;
     }
@@ -521,15 +884,28 @@ cudaError_t launch_sample_of(const SampleArgs &args, cudaStream_t stream) {
     attribute[0].val.clusterDim.z = 1;
     config.attrs = attribute;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, sample_kernel<T>, args, slice, on_chip ? 1u : 0u);
+    return cudaLaunchKernelEx(&config, sample_kernel<T, ON_CHIP>, args, slice);
+}
+
+template <typename T>
+cudaError_t launch_sample_of(const SampleArgs &args, int sm_count, cudaStream_t stream) {
+    // blocks per row: at least 4096 logits each, 8 at most
+    uint32_t blocks = 1;
+    while (blocks < kMostBlocks && args.vocab / (2 * blocks) >= 4096) blocks *= 2;
+    const uint32_t slice = ceil_div(args.vocab, blocks);
+    const size_t slice_bytes = (size_t)slice * sizeof(T) + 64;
+    const size_t smem = sizeof(SampleShared) + ((size_t)slice * sizeof(T) / 16 / kTileWords + 3) * 8;
+    if (slice_bytes <= kSliceBytes && (uint64_t)args.rows * blocks <= (uint64_t)sm_count)
+        return launch_sample_as<T, true>(args, blocks, slice, smem + slice_bytes, stream);
+    return launch_sample_as<T, false>(args, blocks, slice, smem, stream);
 }
 
 }  // namespace
 
-cudaError_t launch_sample(const SampleArgs &args, cudaStream_t stream) {
-    if (args.dtype == kF32) return launch_sample_of<float>(args, stream);
-    if (args.dtype == kBF16) return launch_sample_of<__nv_bfloat16>(args, stream);
-    return launch_sample_of<__half>(args, stream);
+cudaError_t launch_sample(const SampleArgs &args, int sm_count, cudaStream_t stream) {
+    if (args.dtype == kF32) return launch_sample_of<float>(args, sm_count, stream);
+    if (args.dtype == kBF16) return launch_sample_of<__nv_bfloat16>(args, sm_count, stream);
+    return launch_sample_of<__half>(args, sm_count, stream);
 }
 
 }  // namespace q4b

@@ -83,14 +83,16 @@ def check(q4b, ctx, logits, dtype="f32", u=None, seed=0, **rules):
         want, probability, margin = reference(held[r], float(u[r]), *(
             float(rule[name][r]) if name in rule else default
             for name, default in (("temperature", 1.0), ("top_k", 0), ("top_p", 1.0), ("min_p", 0.0))))
-        # The device's weights are whole units of 2^-42 of the largest one's, which exp itself hardly adds to: a running sum
-        # over n tokens is off by n 2^-43, relative to a total of at least one unit of the largest weight.  Where the
-        # definition itself is nearer to a border than that, either neighbour is right.
-        if margin <= vocab * 2.0 ** -42:
+        # A weight on the device is a whole number of units of 2^-42 of the largest one's (half a unit off), made from a
+        # table entry rounded to 2^-31 (half of that, of at least one half), a sum with the rest's product rounded to
+        # 2^-31, and a cubic in fp32 whose value is below 2^-9 (four roundings): 2^-31 + 2^-31 + 2^-31 < 2^-29 of it in
+        # all.  So a running sum of n is off by 2^-29 of itself and n 2^-43 units of the largest weight, and where the
+        # definition is nearer to a border than twice that, either neighbour is right.
+        if margin <= 2.0 ** -28 + vocab * 2.0 ** -42:
             continue
         assert tokens[r] == want, (r, tokens[r], want, margin)
-        # fp32's rounding, and half a unit of the weight itself
-        assert abs(share[r] - probability) <= 2.0 ** -24 * probability + vocab * 2.0 ** -42 + 2.0 ** -149, (r, share[r], probability)
+        # fp32's rounding, and the errors of a weight and of the sum
+        assert abs(share[r] - probability) <= (2.0 ** -24 + 2.0 ** -28) * probability + vocab * 2.0 ** -42 + 2.0 ** -149, (r, share[r], probability)
 
 
 def logits_of(rng, rows, vocab, spread=2.0):
