@@ -52,7 +52,7 @@ struct SampleShared {
     uint64_t parts[3][kMostBlocks];        // sums of the blocks' shares of the bins
     uint64_t warp_values[kSampleWarps];
     float warp_high[kSampleWarps], warp_low[kSampleWarps];
-    uint32_t first, listed, low_bin, high_bin, found_count, fine_bin, fine_count;
+    uint32_t first, listed, own_listed, low_bin, high_bin, found_count, fine_bin, fine_count;
     uint64_t found_before, cut;
     uint64_t span_low[kMostBlocks], span_high[kMostBlocks];
     uint32_t count[kBins];
@@ -60,7 +60,7 @@ struct SampleShared {
         uint64_t list[kListed];            // composites
         uint64_t mass[kBins];
     };
-    uint64_t sums[kListed];
+    uint64_t sums[kListed];                // their weights; before that, what this block puts on the list
 };
 
 // 2^(-j / 256), by repeated multiplication in fp64 (256 roundings of 2^-53 each)
@@ -88,10 +88,11 @@ __device__ inline float as_float(float x) { return x; }
 __device__ inline float as_float(__half x) { return __half2float(x); }
 __device__ inline float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// NaN counts as -infinity, both zeros are one number
+// NaN counts as -infinity, both zeros are one number: in a composite; comparisons, weights (a NaN's is 0) and bins (the
+// last) see to it by themselves
 __device__ inline float tidy(float x) { return x != x ? -INFINITY : x + 0.0f; }
 __device__ inline uint64_t composite(float x, uint32_t index) {
-    const uint32_t bits = __float_as_uint(x);
+    const uint32_t bits = __float_as_uint(tidy(x));
     const uint32_t ordered = bits & 0x80000000u ? ~bits : bits | 0x80000000u;
     return (uint64_t)ordered << 32 | (uint32_t)~index;
 }
@@ -155,7 +156,7 @@ struct Slice {
     const T *data;
     uint32_t begin, size, head, words, tail;
     static constexpr uint32_t kWord = 16 / sizeof(T);
-    __device__ inline float at(uint32_t i) const { return tidy(as_float(data[i])); }
+    __device__ inline float at(uint32_t i) const { return as_float(data[i]); }
     __device__ inline uint32_t tiles() const { return (words + kTileWords - 1) / kTileWords; }
     __device__ inline void split(uint32_t skew) {
         head = min(size, skew == 0 ? 0u : (16u - skew) / (uint32_t)sizeof(T));
@@ -175,7 +176,7 @@ struct Slice {
             if (w < words) {
                 const T *x = reinterpret_cast<const T *>(&word);
 #pragma unroll
-                for (uint32_t j = 0; j < kWord; ++j) f(tidy(as_float(x[j])), head + w * kWord + j);
+                for (uint32_t j = 0; j < kWord; ++j) f(as_float(x[j]), head + w * kWord + j);
             }
         }
     }
@@ -247,21 +248,57 @@ __device__ inline uint32_t my_bin(cg::cluster_group &cluster, uint32_t bins) {
     const uint32_t each = bins / cluster.num_blocks();
     return threadIdx.x < each ? cluster.block_rank() * each + threadIdx.x : 0xffffffffu;
 }
-__device__ inline uint32_t count_of(cg::cluster_group &cluster, SampleShared &sh, uint32_t bin) {
-    uint32_t sum = 0;
-    if (bin != 0xffffffffu)
-        for (uint32_t r = 0; r < cluster.num_blocks(); ++r) sum += cluster.map_shared_rank(&sh, r)->count[bin];
+template <typename V, typename F>
+__device__ inline V over_blocks(cg::cluster_group &cluster, SampleShared &sh, bool any, F f) {
+    V each[kMostBlocks], sum = 0;  // a round trip for all of them, not one each
+#pragma unroll
+    for (uint32_t r = 0; r < kMostBlocks; ++r) each[r] = any && r < cluster.num_blocks() ? f(cluster.map_shared_rank(&sh, r)) : 0;
+#pragma unroll
+    for (uint32_t r = 0; r < kMostBlocks; ++r) sum += each[r];
     return sum;
 }
+__device__ inline uint32_t count_of(cg::cluster_group &cluster, SampleShared &sh, uint32_t bin) {
+    return over_blocks<uint32_t>(cluster, sh, bin != 0xffffffffu, [&](const SampleShared *other) { return other->count[bin]; });
+}
 __device__ inline uint64_t mass_of(cg::cluster_group &cluster, SampleShared &sh, uint32_t bin) {
-    uint64_t sum = 0;
-    if (bin != 0xffffffffu)
-        for (uint32_t r = 0; r < cluster.num_blocks(); ++r) sum += cluster.map_shared_rank(&sh, r)->mass[bin];
-    return sum;
+    return over_blocks<uint64_t>(cluster, sh, bin != 0xffffffffu, [&](const SampleShared *other) { return other->mass[bin]; });
 }
 __device__ inline uint64_t reach_of(float share, uint64_t total) {
     const double reach = ceil((double)fmaxf(share, 0.0f) * (double)total);
     return reach < 1.0 ? 1ull : (uint64_t)reach;
+}
+
+// The elements that `wanted` names, as composites in the list of the cluster's first block; how many there are, or
+// 0xffffffff when they are too many for it.  A block lists its own first: a place in another block's list is a round trip.
+template <typename T, typename F>
+__device__ uint32_t gather(cg::cluster_group &cluster, SampleShared &sh, const Slice<T> &slice, F wanted) {
+    if (threadIdx.x == 0) sh.own_listed = 0;
+    __syncthreads();
+    slice.each([&](float x, uint32_t i) {
+        if (wanted(x, i)) {
+            const uint32_t place = atomicAdd(&sh.own_listed, 1u);
+            if (place < kListed) sh.sums[place] = composite(x, slice.begin + i);
+        }
+    });
+    __syncthreads();
+    const uint32_t own = sh.own_listed, blocks = cluster.num_blocks(), rank = cluster.block_rank();
+    if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->span_high[rank] = own;
+    cluster.sync();
+    uint32_t before = 0, all = 0;
+    for (uint32_t r = 0; r < blocks; ++r) {
+        const uint32_t count = (uint32_t)sh.span_high[r];
+        if (r < rank) before += count;
+        all += count;
+    }
+    if (all > kListed) {
+        cluster.sync();
+        return 0xffffffffu;
+    }
+    SampleShared *leader = cluster.map_shared_rank(&sh, 0);
+    for (uint32_t i = threadIdx.x; i < own; i += kSampleThreads) leader->list[before + i] = sh.sums[i];
+    if (rank == 0 && threadIdx.x == 0) sh.listed = all;
+    cluster.sync();
+    return all;
 }
 
 // The composite of the last element that stays, over the whole cluster, in every case.  By count: the `wanted`-th element
@@ -283,7 +320,6 @@ __device__ __noinline__ uint64_t find_cut(cg::cluster_group &cluster, SampleShar
             sh.count[b] = 0;
             if (MASS) sh.mass[b] = 0;
         }
-        if (threadIdx.x == 0) sh.listed = 0;
         __syncthreads();
         slice.each([&](float x, uint32_t i) {
             const uint64_t c = composite(x, slice.begin + i);
@@ -315,12 +351,10 @@ __device__ __noinline__ uint64_t find_cut(cg::cluster_group &cluster, SampleShar
         before = sh.found_before;
         if (border_count <= kListed) {
             // gather the bin in the first block and rank it there
-            SampleShared *leader = cluster.map_shared_rank(&sh, 0);
-            slice.each([&](float x, uint32_t i) {
+            gather(cluster, sh, slice, [&](float x, uint32_t i) {
                 const uint64_t c = composite(x, slice.begin + i);
-                if (in_span(c) && bin_of(x, c) == border) leader->list[atomicAdd(&leader->listed, 1u)] = c;
+                return in_span(c) && bin_of(x, c) == border;
             });
-            cluster.sync();
             if (rank == 0) {
                 const uint32_t n = sh.listed;
                 if (MASS) {
@@ -399,7 +433,7 @@ __device__ inline uint64_t target_of(float uniform, uint64_t total) {
 // All that matter are in this block's list: cut them, draw, and answer.  `mass` is the sum that top-p is a share of, or 0
 // where it is the sum of the first k.
 __device__ __noinline__ void finish_list(const SampleArgs &p, uint32_t row, SampleShared &sh, const Weigh &weigh, uint32_t k,
-                                         float share, uint64_t mass, uint64_t least) {
+                                         float share, uint64_t mass, uint64_t least, float uniform) {
     const uint32_t n = sh.listed;
     uint32_t size = 32;
     while (size < n) size *= 2;
@@ -407,40 +441,48 @@ __device__ __noinline__ void finish_list(const SampleArgs &p, uint32_t row, Samp
     __syncthreads();
     if (n > kSampleThreads) block_sort<false>(sh.list, n);
     const uint32_t first = k != 0 && k < n ? k : n;
-    const float uniform = p.uniform[row];
     if (n <= kSampleThreads) {
-        // an element per thread, ranked against all others: fewer steps than sorting twice
+        // an element per thread, sorted by exchanges within the warps as far as those reach
         const uint32_t i = threadIdx.x;
-        const uint64_t own = i < n ? sh.list[i] : 0, weight = i < n ? weigh.of(logit_of(own)) : 0;
-        if (i < n) sh.sums[i] = weight;
-        __syncthreads();
-        uint32_t place = 0;
-        uint64_t above = 0;
-        if (i < n) {
-#pragma unroll 4
-            for (uint32_t j = 0; j < n; ++j) {
-                if (sh.list[j] > own) {
-                    ++place;
-                    above += sh.sums[j];
+        uint64_t own = i < size ? sh.list[i] : 0;
+#pragma unroll 1
+        for (uint32_t k2 = 2; k2 <= size; k2 *= 2) {
+#pragma unroll 1
+            for (uint32_t j = k2 / 2; j > 0; j /= 2) {
+                uint64_t other;
+                if (j >= 32) {
+                    __syncthreads();
+                    sh.list[i] = own;
+                    __syncthreads();
+                    other = sh.list[i ^ j];
+                } else {
+                    other = __shfl_xor_sync(0xffffffffu, own, j);
                 }
+                const bool larger = ((i & j) == 0) == ((i & k2) == 0);
+                own = (own > other) == larger ? own : other;
             }
         }
-        bool stays = i < n && place < first;
-        const uint64_t whole_sum = mass != 0 || !(share < 1.0f) ? mass : block_sum(stays ? weight : 0, sh.warp_values);
-        if (share < 1.0f) stays = stays && above < reach_of(share, whole_sum);
-        stays = stays && weight >= least;
+        const uint64_t weight = i < n ? weigh.of(logit_of(own)) : 0;
+        uint64_t above;
+        const uint64_t sum_first = block_scan(i < first ? weight : 0, sh.warp_values, above);
+        bool stays = i < first && weight >= least;
+        if (share < 1.0f) stays = stays && above < reach_of(share, mass != 0 ? mass : sum_first);
         const uint64_t total = block_sum(stays ? weight : 0, sh.warp_values);
-        __syncthreads();
-        if (i < n) sh.sums[i] = stays ? weight : 0;
+        const uint32_t m = (uint32_t)__syncthreads_count(stays);  // a prefix
+        const uint32_t index = index_of(own);
+        if (i < m) {
+            sh.sums[i] = weight;
+            sh.count[i] = index;
+        }
         __syncthreads();
         if (!stays) return;
         uint64_t running = 0;
 #pragma unroll 4
-        for (uint32_t j = 0; j < n; ++j)
-            if ((uint32_t)sh.list[j] > (uint32_t)own) running += sh.sums[j];  // a smaller index: its complement is larger
+        for (uint32_t j = 0; j < m; ++j)
+            if (sh.count[j] < index) running += sh.sums[j];
         const uint64_t target = target_of(uniform, total);
         if (running <= target && running + weight > target) {
-            p.tokens[row] = index_of(own);
+            p.tokens[row] = index;
             if (p.probabilities != nullptr) p.probabilities[row] = (float)((double)weight / (double)total);
         }
         return;
@@ -508,6 +550,13 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t row = blockIdx.x / blocks, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 
+    // asked for first, needed late
+    const float temperature = p.temperature != nullptr ? p.temperature[row] : 1.0f;
+    const uint32_t asked_k = p.top_k != nullptr ? p.top_k[row] : 0;
+    const float share = p.top_p != nullptr ? p.top_p[row] : 1.0f;
+    const float floor_p = p.min_p != nullptr ? p.min_p[row] : 0.0f;
+    const float uniform = p.uniform[row];
+
     Slice<T> slice;
     slice.begin = min(rank * slice_size, p.vocab);
     slice.size = min(slice_size, p.vocab - slice.begin);
@@ -517,7 +566,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     cg::cluster_group::arrival_token running_token = cluster.barrier_arrive();
 
     // ---- load: extremes on the way ----
-    float high = -INFINITY, low = INFINITY;
+    float high = -INFINITY, low = INFINITY;  // first of what this thread reads
     auto look = [&](float x, uint32_t) {
         high = fmaxf(high, x);
         if (x > -INFINITY) low = fminf(low, x);
@@ -540,7 +589,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
                     to[w0 + u * kSampleThreads] = word[u];
                     const T *x = reinterpret_cast<const T *>(&word[u]);
 #pragma unroll
-                    for (uint32_t j = 0; j < Slice<T>::kWord; ++j) look(tidy(as_float(x[j])), 0);
+                    for (uint32_t j = 0; j < Slice<T>::kWord; ++j) look(as_float(x[j]), 0);
                 }
             }
         }
@@ -553,6 +602,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     } else {
         slice.each(look);
     }
+    const float own_high = high;
     if (threadIdx.x < 256) sh.power[threadIdx.x] = kPowers.entry[threadIdx.x];
     for (uint32_t b = threadIdx.x; b < kBins; b += kSampleThreads) sh.count[b] = 0;
     if (threadIdx.x == 0) {
@@ -591,7 +641,6 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         high = fmaxf(high, sh.high[r]);
         low = fminf(low, sh.low[r]);
     }
-    const float temperature = p.temperature != nullptr ? p.temperature[row] : 1.0f;
     if (high == -INFINITY) {
         if (rank == 0 && threadIdx.x == 0) {
             p.tokens[row] = 0xffffffffu;
@@ -621,13 +670,40 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     weigh.rate_low = weigh.rate < 3.0e38f ? (float)(rate - (double)weigh.rate) : 0.0f;
     const uint32_t bins = min(kBins, blocks * kSampleThreads);
     const float last_bin = (float)(bins - 1), to_bin = last_bin / fmaxf(high - low, 1e-30f);
-    const uint32_t k = p.top_k != nullptr && p.top_k[row] < p.vocab ? p.top_k[row] : 0;
-    const float share = p.top_p != nullptr ? p.top_p[row] : 1.0f;
-    const float floor_p = p.min_p != nullptr ? p.min_p[row] : 0.0f;
+    const uint32_t k = asked_k < p.vocab ? asked_k : 0;
     // the least weight that stays, in units (a NaN is none)
     const uint64_t least = floor_p > 0.0f ? (uint64_t)ceil((double)fminf(floor_p, 1.0f) * (double)kOne) : 0;
 
     uint64_t cut = 0;
+    if (k != 0 && k <= kListed / 2) {
+        // ---- few by count ----
+        // The k-th largest of the threads' own maxima is at most the k-th largest of all, and hardly smaller while k is a
+        // fraction of the threads: bins of one element per thread tell how far down the list has to go.
+        if (own_high > -INFINITY) atomicAdd(&sh.count[whole(place_of(own_high, high, to_bin, last_bin))], 1u);
+        if (threadIdx.x == 0) sh.found_count = 0;
+        cluster.sync();
+        const uint32_t bin = my_bin(cluster, bins), number = count_of(cluster, sh, bin);
+        uint64_t before = tell_parts(cluster, sh, 0, number), all;
+        cluster.sync();  // the bins have been read everywhere
+        before += sum_parts(cluster, sh, 0, all);
+        if (number != 0 && before < k && before + number >= k) {
+            for (uint32_t r = 0; r < blocks; ++r) {
+                SampleShared *other = cluster.map_shared_rank(&sh, r);
+                other->high_bin = bin;
+                other->found_count = 1;
+            }
+        }
+        cluster.sync();
+        if (sh.found_count != 0) {  // fewer threads than k otherwise
+            const float end = (float)(sh.high_bin + 1);
+            if (gather(cluster, sh, slice, [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; }) <= kListed) {
+                if (rank == 0) finish_list(p, row, sh, weigh, k, share, 0, least, uniform);
+                return;
+            }
+        }
+        for (uint32_t b = threadIdx.x; b < bins; b += kSampleThreads) sh.count[b] = 0;
+        __syncthreads();
+    }
     if (k != 0 || share < 1.0f) {
         // ---- counts ----
         const bool add = k == 0;  // top-p alone is a share of everything
@@ -692,13 +768,9 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         const uint32_t low_bin = sh.low_bin, high_bin = sh.high_bin, down_to = sh.found_count;
         if (down_to != 0 && down_to <= kListed) {
             // ---- few stay ----
-            SampleShared *leader = cluster.map_shared_rank(&sh, 0);
             const float end = (float)(high_bin + 1);
-            slice.each([&](float x, uint32_t i) {
-                if (place_of(x, high, to_bin, last_bin) < end) leader->list[atomicAdd(&leader->listed, 1u)] = composite(x, slice.begin + i);
-            });
-            cluster.sync();
-            if (rank == 0) finish_list(p, row, sh, weigh, k, share, everything, least);
+            gather(cluster, sh, slice, [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; });
+            if (rank == 0) finish_list(p, row, sh, weigh, k, share, everything, least, uniform);
             return;
         }
         if (add) {
@@ -743,13 +815,10 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             const uint32_t border = sh.fine_bin, border_count = sh.fine_count;
             const uint64_t before = sh.found_before;
             if (border_count != 0 && border_count <= kListed) {
-                SampleShared *leader = cluster.map_shared_rank(&sh, 0);
-                slice.each([&](float x, uint32_t i) {
+                gather(cluster, sh, slice, [&](float x, uint32_t) {
                     const float v = place_of(x, high, to_bin, last_bin);
-                    if (v >= first && v < end && fine_bin(v) == border)
-                        leader->list[atomicAdd(&leader->listed, 1u)] = composite(x, slice.begin + i);
+                    return v >= first && v < end && fine_bin(v) == border;
                 });
-                cluster.sync();
                 if (rank == 0) {
                     const uint32_t n = sh.listed;
                     for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) sh.sums[i] = weigh.of(logit_of(sh.list[i]));
@@ -817,7 +886,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         if (r < rank) before += sh.total[r];
         total += sh.total[r];
     }
-    const uint64_t target = target_of(p.uniform[row], total);
+    const uint64_t target = target_of(uniform, total);
     if (target < before || target >= before + mine || warp != 0) return;
     // the tile, 32 at a time
     uint64_t running = before;
