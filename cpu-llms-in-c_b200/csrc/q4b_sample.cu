@@ -35,9 +35,8 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr uint32_t kSampleThreads = 512;
-constexpr uint32_t kSampleWarps = kSampleThreads / 32;
-constexpr uint32_t kBins = 2048;           // at most: 512 per block of the cluster, a thread each
+constexpr uint32_t kMostWarps = 32;
+constexpr uint32_t kBins = 2048;           // at most: a thread of the cluster for each
 constexpr uint32_t kMostBlocks = 8;        // thread blocks of a row
 constexpr uint32_t kListed = 2048;         // elements that one block puts in order
 constexpr uint32_t kTileRows4 = 4;         // 16-byte words of a tile: 4 per lane of a warp
@@ -50,8 +49,8 @@ struct SampleShared {
     float high[kMostBlocks], low[kMostBlocks];
     uint64_t total[kMostBlocks];
     uint64_t parts[3][kMostBlocks];        // sums of the blocks' shares of the bins
-    uint64_t warp_values[kSampleWarps];
-    float warp_high[kSampleWarps], warp_low[kSampleWarps];
+    uint64_t warp_values[kMostWarps];
+    float warp_high[kMostWarps], warp_low[kMostWarps];
     uint32_t first, listed, own_listed, low_bin, high_bin, found_count, fine_bin, fine_count;
     uint64_t found_before, cut;
     uint64_t span_low[kMostBlocks], span_high[kMostBlocks];
@@ -129,7 +128,7 @@ __device__ inline uint64_t block_max(uint64_t x, uint64_t *scratch) {
     x = warp_max(x);
     if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = x;
     __syncthreads();
-    x = warp_max(scratch[threadIdx.x & (kSampleWarps - 1)]);
+    x = warp_max((threadIdx.x & 31) < blockDim.x / 32 ? scratch[threadIdx.x & 31] : 0);
     __syncthreads();
     return x;
 }
@@ -139,8 +138,8 @@ __device__ inline uint64_t block_scan(uint64_t x, uint64_t *scratch, uint64_t &b
     const uint64_t inclusive = warp_inclusive(x);
     if (lane == 31) scratch[warp] = inclusive;
     __syncthreads();
-    const uint64_t warps = warp_inclusive(lane < kSampleWarps ? scratch[lane] : 0);
-    const uint64_t total = __shfl_sync(0xffffffffu, warps, kSampleWarps - 1);
+    const uint64_t warps = warp_inclusive(lane < blockDim.x / 32 ? scratch[lane] : 0);
+    const uint64_t total = __shfl_sync(0xffffffffu, warps, 31);
     before = inclusive - x + (warp > 0 ? __shfl_sync(0xffffffffu, warps, warp - 1) : 0);
     __syncthreads();
     return total;
@@ -184,7 +183,7 @@ struct Slice {
     template <typename F> __device__ inline void each(F f) const {
         const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll 1
-        for (uint32_t t = warp; t < tiles(); t += kSampleWarps) tile(t, f);
+        for (uint32_t t = warp; t < tiles(); t += (blockDim.x / 32)) tile(t, f);
         if (warp == 0 && lane < head + tail) {
             const uint32_t i = lane < head ? lane : size - tail + (lane - head);
             f(at(i), i);
@@ -192,10 +191,10 @@ struct Slice {
     }
 };
 
-// Weights by the distance to the largest logit.
+// Weights by the distance to the largest logit: about 45 instructions, which are what a pass costs.
 struct Weigh {
     const uint2 *power;
-    float high, rate, rate_low;  // log2(e) / temperature = rate + rate_low
+    float high, rate, rate_low;  // log2(e) / temperature = rate + rate_low, finite
     // of distance + distance_low >= 0; beyond 2^-43, overflow and NaN are nothing
     __device__ inline uint64_t at(float distance, float distance_low) const {
         const float y = distance * rate;
@@ -207,9 +206,9 @@ struct Weigh {
         const float q = rest * -0.693147180559945309f;
         const float more = q * fmaf(q, fmaf(q, 0.16666667f, 0.5f), 1.0f);  // 2^-rest - 1; q^4 / 24 < 2^-42
         const uint2 base = power[k & 255u];
-        const uint32_t add = __float_as_uint(fmaf(__uint_as_float(base.y), more, 12582912.0f)) - 0x4b400000u;
+        const uint32_t value = base.x + __float_as_uint(fmaf(__uint_as_float(base.y), more, 12582912.0f)) - 0x4b400000u;
         const uint32_t n = k >> 8;
-        return (((uint64_t)(base.x + add) << 11) + ((1ull << n) >> 1)) >> n;
+        return (((uint64_t)value << 11) + ((1ull << n) >> 1)) >> n;
     }
     __device__ inline uint64_t of(float x) const {
         if (x == high) return kOne;
@@ -295,7 +294,7 @@ __device__ uint32_t gather(cg::cluster_group &cluster, SampleShared &sh, const S
         return 0xffffffffu;
     }
     SampleShared *leader = cluster.map_shared_rank(&sh, 0);
-    for (uint32_t i = threadIdx.x; i < own; i += kSampleThreads) leader->list[before + i] = sh.sums[i];
+    for (uint32_t i = threadIdx.x; i < own; i += blockDim.x) leader->list[before + i] = sh.sums[i];
     if (rank == 0 && threadIdx.x == 0) sh.listed = all;
     cluster.sync();
     return all;
@@ -316,7 +315,7 @@ __device__ __noinline__ uint64_t find_cut(cg::cluster_group &cluster, SampleShar
     };
     auto in_span = [&](uint64_t c) { return c >= span_low && c <= span_high; };
     for (;;) {
-        for (uint32_t b = threadIdx.x; b < kBins; b += kSampleThreads) {
+        for (uint32_t b = threadIdx.x; b < kBins; b += blockDim.x) {
             sh.count[b] = 0;
             if (MASS) sh.mass[b] = 0;
         }
@@ -358,10 +357,10 @@ __device__ __noinline__ uint64_t find_cut(cg::cluster_group &cluster, SampleShar
             if (rank == 0) {
                 const uint32_t n = sh.listed;
                 if (MASS) {
-                    for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) sh.sums[i] = weigh.of(logit_of(sh.list[i]));
+                    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) sh.sums[i] = weigh.of(logit_of(sh.list[i]));
                     __syncthreads();
                 }
-                for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) {
+                for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
                     const uint64_t c = sh.list[i];
                     uint64_t above = before;
                     for (uint32_t j = 0; j < n; ++j) {
@@ -411,7 +410,7 @@ __device__ void block_sort(V *values, uint32_t n) {
     while (size < n) size *= 2;
     for (uint32_t k = 2; k <= size; k *= 2) {
         for (uint32_t j = k / 2; j > 0; j /= 2) {
-            for (uint32_t pair = threadIdx.x; pair < size / 2; pair += kSampleThreads) {
+            for (uint32_t pair = threadIdx.x; pair < size / 2; pair += blockDim.x) {
                 const uint32_t i = 2 * pair - (pair & (j - 1)), other = i + j;
                 const V x = values[i], y = values[other];
                 if ((x > y) == (((i & k) == 0) != UP ? false : true)) {
@@ -437,11 +436,11 @@ __device__ __noinline__ void finish_list(const SampleArgs &p, uint32_t row, Samp
     const uint32_t n = sh.listed;
     uint32_t size = 32;
     while (size < n) size *= 2;
-    for (uint32_t i = n + threadIdx.x; i < size; i += kSampleThreads) sh.list[i] = 0;
+    for (uint32_t i = n + threadIdx.x; i < size; i += blockDim.x) sh.list[i] = 0;
     __syncthreads();
-    if (n > kSampleThreads) block_sort<false>(sh.list, n);
+    if (n > blockDim.x) block_sort<false>(sh.list, n);
     const uint32_t first = k != 0 && k < n ? k : n;
-    if (n <= kSampleThreads) {
+    if (n <= blockDim.x) {
         // an element per thread, sorted by exchanges within the warps as far as those reach
         const uint32_t i = threadIdx.x;
         uint64_t own = i < size ? sh.list[i] : 0;
@@ -487,27 +486,21 @@ __device__ __noinline__ void finish_list(const SampleArgs &p, uint32_t row, Samp
         }
         return;
     }
-    // in order: running weights, four neighbours per thread
-    uint64_t weight[4], own = 0, running;
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-        const uint32_t i = 4 * threadIdx.x + e;
-        weight[e] = i < n ? weigh.of(logit_of(sh.list[i])) : 0;
-        own += weight[e];
-    }
-    block_scan(own, sh.warp_values, running);
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-        running += weight[e];
-        sh.sums[4 * threadIdx.x + e] = running;
+    // in order: running weights, each thread a run of neighbours
+    const uint32_t each = kListed / blockDim.x, i0 = threadIdx.x * each;
+    uint64_t sum = 0, running;
+    for (uint32_t i = i0; i < min(n, i0 + each); ++i) sum += weigh.of(logit_of(sh.list[i]));
+    block_scan(sum, sh.warp_values, running);
+    for (uint32_t i = i0; i < min(n, i0 + each); ++i) {
+        running += weigh.of(logit_of(sh.list[i]));
+        sh.sums[i] = running;
     }
     __syncthreads();
+    auto weight_of = [&](uint32_t i) { return sh.sums[i] - (i > 0 ? sh.sums[i - 1] : 0); };
     const uint64_t wanted = share < 1.0f ? reach_of(share, mass != 0 ? mass : sh.sums[first - 1]) : ~0ull;
     uint32_t stay = 0;  // how many stay: a prefix
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-        const uint32_t i = 4 * threadIdx.x + e;
-        if (i < first && sh.sums[i] - weight[e] < wanted && weight[e] >= least) ++stay;
+    for (uint32_t i = i0; i < min(first, i0 + each); ++i) {
+        if (sh.sums[i] - weight_of(i) < wanted && weight_of(i) >= least) ++stay;
     }
     const uint32_t m = (uint32_t)block_sum(stay, sh.warp_values);
     const uint64_t total = sh.sums[m - 1];
@@ -515,33 +508,27 @@ __device__ __noinline__ void finish_list(const SampleArgs &p, uint32_t row, Samp
     uint32_t *const by_index = sh.count;
     size = 32;
     while (size < m) size *= 2;
-    for (uint32_t i = threadIdx.x; i < size; i += kSampleThreads)
+    for (uint32_t i = threadIdx.x; i < size; i += blockDim.x)
         by_index[i] = i < m ? index_of(sh.list[i]) << 11 | i : 0xffffffffu;
     __syncthreads();
     block_sort<true>(by_index, m);
-    own = 0;
-    uint32_t place[4];
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-        const uint32_t i = 4 * threadIdx.x + e;
-        place[e] = i < m ? by_index[i] & (kListed - 1) : 0;
-        weight[e] = i < m ? sh.sums[place[e]] - (place[e] > 0 ? sh.sums[place[e] - 1] : 0) : 0;
-        own += weight[e];
-    }
-    block_scan(own, sh.warp_values, running);
+    sum = 0;
+    for (uint32_t i = i0; i < min(m, i0 + each); ++i) sum += weight_of(by_index[i] & (kListed - 1));
+    block_scan(sum, sh.warp_values, running);
     const uint64_t target = target_of(uniform, total);
-#pragma unroll
-    for (uint32_t e = 0; e < 4; ++e) {
-        if (running <= target && running + weight[e] > target) {
-            p.tokens[row] = index_of(sh.list[place[e]]);
-            if (p.probabilities != nullptr) p.probabilities[row] = (float)((double)weight[e] / (double)total);
+    for (uint32_t i = i0; i < min(m, i0 + each); ++i) {
+        const uint32_t place = by_index[i] & (kListed - 1);
+        const uint64_t weight = weight_of(place);
+        if (running <= target && running + weight > target) {
+            p.tokens[row] = index_of(sh.list[place]);
+            if (p.probabilities != nullptr) p.probabilities[row] = (float)((double)weight / (double)total);
         }
-        running += weight[e];
+        running += weight;
     }
 }
 
-template <typename T, bool ON_CHIP>
-__global__ void __launch_bounds__(kSampleThreads, ON_CHIP ? 1 : 2)
+template <typename T, bool ON_CHIP, int THREADS>
+__global__ void __launch_bounds__(THREADS, ON_CHIP ? 1 : 1024 / THREADS)
 sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     cg::cluster_group cluster = cg::this_cluster();
     extern __shared__ __align__(16) uint8_t sample_smem[];
@@ -567,26 +554,29 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
 
     // ---- load: extremes on the way ----
     float high = -INFINITY, low = INFINITY;  // first of what this thread reads
+    const bool binned = asked_k != 0 || share < 1.0f;  // the smallest only spaces the bins
     auto look = [&](float x, uint32_t) {
         high = fmaxf(high, x);
-        if (x > -INFINITY) low = fminf(low, x);
+        if (binned && x > -INFINITY) low = fminf(low, x);
     };
-    if (ON_CHIP) {
+    {
         // the copy starts at the same place within 16 bytes as the original, so whole words move
         uint8_t *held = reinterpret_cast<uint8_t *>(tiles + slice.tiles() + 2);
         held += ((16u - (uint32_t)(reinterpret_cast<uintptr_t>(held) & 15u)) & 15u) + skew;
         T *const copy = reinterpret_cast<T *>(held);
         const uint4 *const from = reinterpret_cast<const uint4 *>(slice.data + slice.head);
         uint4 *const to = reinterpret_cast<uint4 *>(copy + slice.head);
-        for (uint32_t w0 = threadIdx.x; w0 < slice.words; w0 += 8 * kSampleThreads) {
-            uint4 word[8];
+        constexpr uint32_t kAtOnce = ON_CHIP ? 8 : 6;  // words on their way per thread
+#pragma unroll 1
+        for (uint32_t w0 = threadIdx.x; w0 < slice.words; w0 += kAtOnce * blockDim.x) {
+            uint4 word[kAtOnce];
 #pragma unroll
-            for (uint32_t u = 0; u < 8; ++u)
-                if (w0 + u * kSampleThreads < slice.words) word[u] = __ldcs(from + w0 + u * kSampleThreads);
+            for (uint32_t u = 0; u < kAtOnce; ++u)
+                if (w0 + u * blockDim.x < slice.words) word[u] = ON_CHIP ? __ldcs(from + w0 + u * blockDim.x) : from[w0 + u * blockDim.x];
 #pragma unroll
-            for (uint32_t u = 0; u < 8; ++u) {
-                if (w0 + u * kSampleThreads < slice.words) {
-                    to[w0 + u * kSampleThreads] = word[u];
+            for (uint32_t u = 0; u < kAtOnce; ++u) {
+                if (w0 + u * blockDim.x < slice.words) {
+                    if (ON_CHIP) to[w0 + u * blockDim.x] = word[u];
                     const T *x = reinterpret_cast<const T *>(&word[u]);
 #pragma unroll
                     for (uint32_t j = 0; j < Slice<T>::kWord; ++j) look(as_float(x[j]), 0);
@@ -595,16 +585,14 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         }
         if (threadIdx.x < slice.head + slice.tail) {
             const uint32_t i = threadIdx.x < slice.head ? threadIdx.x : slice.size - slice.tail + threadIdx.x - slice.head;
-            copy[i] = slice.data[i];
+            if (ON_CHIP) copy[i] = slice.data[i];
             look(slice.at(i), 0);
         }
-        slice.data = copy;
-    } else {
-        slice.each(look);
+        if (ON_CHIP) slice.data = copy;
     }
     const float own_high = high;
-    if (threadIdx.x < 256) sh.power[threadIdx.x] = kPowers.entry[threadIdx.x];
-    for (uint32_t b = threadIdx.x; b < kBins; b += kSampleThreads) sh.count[b] = 0;
+    for (uint32_t j = threadIdx.x; j < 256; j += blockDim.x) sh.power[j] = kPowers.entry[j];
+    for (uint32_t b = threadIdx.x; b < kBins; b += blockDim.x) sh.count[b] = 0;
     if (threadIdx.x == 0) {
         sh.listed = 0;
         sh.first = 0xffffffffu;
@@ -621,10 +609,10 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     __syncthreads();
     cluster.barrier_wait(static_cast<cg::cluster_group::arrival_token &&>(running_token));  // every block of the cluster runs
     if (warp == 0) {
-        high = sh.warp_high[lane & (kSampleWarps - 1)];
-        low = sh.warp_low[lane & (kSampleWarps - 1)];
+        high = lane < blockDim.x / 32 ? sh.warp_high[lane] : -INFINITY;
+        low = lane < blockDim.x / 32 ? sh.warp_low[lane] : INFINITY;
 #pragma unroll
-        for (int d = kSampleWarps / 2; d > 0; d >>= 1) {
+        for (int d = 16; d > 0; d >>= 1) {
             high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
             low = fminf(low, __shfl_xor_sync(0xffffffffu, low, d));
         }
@@ -666,9 +654,9 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     weigh.power = sh.power;
     weigh.high = high;
     const double rate = 1.4426950408889634074 / (double)temperature;
-    weigh.rate = (float)rate;
+    weigh.rate = fminf((float)rate, 3.0e38f);
     weigh.rate_low = weigh.rate < 3.0e38f ? (float)(rate - (double)weigh.rate) : 0.0f;
-    const uint32_t bins = min(kBins, blocks * kSampleThreads);
+    const uint32_t bins = min(kBins, blocks * blockDim.x);
     const float last_bin = (float)(bins - 1), to_bin = last_bin / fmaxf(high - low, 1e-30f);
     const uint32_t k = asked_k < p.vocab ? asked_k : 0;
     // the least weight that stays, in units (a NaN is none)
@@ -701,7 +689,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
                 return;
             }
         }
-        for (uint32_t b = threadIdx.x; b < bins; b += kSampleThreads) sh.count[b] = 0;
+        for (uint32_t b = threadIdx.x; b < bins; b += blockDim.x) sh.count[b] = 0;
         __syncthreads();
     }
     if (k != 0 || share < 1.0f) {
@@ -775,7 +763,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         }
         if (add) {
             // ---- many stay: the bracket by exact weights ----
-            for (uint32_t b = threadIdx.x; b < bins; b += kSampleThreads) {
+            for (uint32_t b = threadIdx.x; b < bins; b += blockDim.x) {
                 sh.count[b] = 0;
                 sh.mass[b] = 0;
             }
@@ -821,9 +809,9 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
                 });
                 if (rank == 0) {
                     const uint32_t n = sh.listed;
-                    for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) sh.sums[i] = weigh.of(logit_of(sh.list[i]));
+                    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) sh.sums[i] = weigh.of(logit_of(sh.list[i]));
                     __syncthreads();
-                    for (uint32_t i = threadIdx.x; i < n; i += kSampleThreads) {
+                    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
                         const uint64_t c = sh.list[i];
                         uint64_t over = before;
 #pragma unroll 4
@@ -859,10 +847,10 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     auto kept = [&](float x, uint32_t i) -> uint64_t {
         if (!all && composite(x, slice.begin + i) < cut) return 0;
         const uint64_t w = weigh.of(x);
-        return w < least ? 0ull : w;
+        return least != 0 && w < least ? 0ull : w;
     };
     const uint32_t word_tiles = slice.tiles(), tile_count = word_tiles + 2;
-    for (uint32_t t = warp; t < tile_count; t += kSampleWarps) {
+    for (uint32_t t = warp; t < tile_count; t += (blockDim.x / 32)) {
         uint64_t sum = 0;
         if (t == 0) {
             if (lane < slice.head) sum = kept(slice.at(lane), lane);
@@ -876,7 +864,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     }
     __syncthreads();
     uint64_t mine = 0;
-    for (uint32_t t = threadIdx.x; t < tile_count; t += kSampleThreads) mine += tiles[t];
+    for (uint32_t t = threadIdx.x; t < tile_count; t += blockDim.x) mine += tiles[t];
     mine = block_sum(mine, sh.warp_values);
     // (the sums of the top-p passes have been read everywhere: a cluster barrier lies between)
     if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->total[rank] = mine;
@@ -931,19 +919,19 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     }
 }
 
-template <typename T, bool ON_CHIP>
+template <typename T, bool ON_CHIP, int THREADS>
 cudaError_t launch_sample_as(const SampleArgs &args, uint32_t blocks, uint32_t slice, size_t smem, cudaStream_t stream) {
     static bool configured[kMaxDevices] = {};
     const int slot = device_slot();
     if (slot < 0 || !configured[slot]) {
         const size_t most = sizeof(SampleShared) + ((1u << 20) / kMostBlocks * 4 / 16 / kTileWords + 3) * 8 + (ON_CHIP ? kSliceBytes : 0);
-        cudaError_t status = cudaFuncSetAttribute(sample_kernel<T, ON_CHIP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+        cudaError_t status = cudaFuncSetAttribute(sample_kernel<T, ON_CHIP, THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
         if (status != cudaSuccess) return status;
         if (slot >= 0) configured[slot] = true;
     }
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(args.rows * blocks);
-    config.blockDim = dim3(kSampleThreads);
+    config.blockDim = dim3(THREADS);
     config.dynamicSmemBytes = smem;
     config.stream = stream;
     cudaLaunchAttribute attribute[1];
@@ -953,7 +941,7 @@ cudaError_t launch_sample_as(const SampleArgs &args, uint32_t blocks, uint32_t s
     attribute[0].val.clusterDim.z = 1;
     config.attrs = attribute;
     config.numAttrs = 1;
-    return cudaLaunchKernelEx(&config, sample_kernel<T, ON_CHIP>, args, slice);
+    return cudaLaunchKernelEx(&config, sample_kernel<T, ON_CHIP, THREADS>, args, slice);
 }
 
 template <typename T>
@@ -965,8 +953,13 @@ cudaError_t launch_sample_of(const SampleArgs &args, int sm_count, cudaStream_t 
     const size_t slice_bytes = (size_t)slice * sizeof(T) + 64;
     const size_t smem = sizeof(SampleShared) + ((size_t)slice * sizeof(T) / 16 / kTileWords + 3) * 8;
     if (slice_bytes <= kSliceBytes && (uint64_t)args.rows * blocks <= (uint64_t)sm_count)
-        return launch_sample_as<T, true>(args, blocks, slice, smem + slice_bytes, stream);
-    return launch_sample_as<T, false>(args, blocks, slice, smem, stream);
+        return launch_sample_as<T, true, 512>(args, blocks, slice, smem + slice_bytes, stream);
+    // Two blocks of 512 threads per SM, or four of 256 whose short phases fill each other's waits: better for a whole
+    // distribution in more than one wave (256 fp32 rows of 248,320: XX us against YY us), worse for the longer chain
+    // of a top-p cut (64 fp16 rows: XX us against YY us).
+    if (args.top_k == nullptr && args.top_p == nullptr && (uint64_t)args.rows * blocks > 2 * (uint64_t)sm_count)
+        return launch_sample_as<T, false, 256>(args, blocks, slice, smem, stream);
+    return launch_sample_as<T, false, 512>(args, blocks, slice, smem, stream);
 }
 
 }  // namespace
