@@ -51,7 +51,7 @@ struct SampleShared {
     uint64_t parts[3][kMostBlocks];        // sums of the blocks' shares of the bins
     uint64_t warp_values[kMostWarps];
     float warp_high[kMostWarps], warp_low[kMostWarps];
-    uint32_t first, listed, own_listed, low_bin, high_bin, found_count, fine_bin, fine_count;
+    uint32_t first, listed, own_listed, low_bin, high_bin, low_before, found_count, fine_bin, fine_count;
     uint64_t found_before, cut;
     uint64_t span_low[kMostBlocks], span_high[kMostBlocks];
     uint32_t count[kBins];
@@ -745,7 +745,10 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         if (number != 0 && (is_low || is_high)) {
             for (uint32_t r = 0; r < blocks; ++r) {
                 SampleShared *other = cluster.map_shared_rank(&sh, r);
-                if (is_low) other->low_bin = bin;
+                if (is_low) {
+                    other->low_bin = bin;
+                    other->low_before = (uint32_t)number_before;
+                }
                 if (is_high) {
                     other->high_bin = bin;
                     other->found_count = (uint32_t)number_before + number;
@@ -753,7 +756,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             }
         }
         cluster.sync();
-        const uint32_t low_bin = sh.low_bin, high_bin = sh.high_bin, down_to = sh.found_count;
+        const uint32_t low_bin = sh.low_bin, high_bin = sh.high_bin, down_to = sh.found_count, low_before = sh.low_before;
         if (down_to != 0 && down_to <= kListed) {
             // ---- few stay ----
             const float end = (float)(high_bin + 1);
@@ -761,7 +764,45 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             if (rank == 0) finish_list(p, row, sh, weigh, k, share, everything, least, uniform);
             return;
         }
-        if (add) {
+        // the first block puts its list in order and finds where the running weight reaches `wanted`
+        auto rank_list = [&](uint64_t before) {
+            if (rank == 0) {
+                const uint32_t n = sh.listed;
+                uint32_t size = 32;
+                while (size < n) size *= 2;
+                for (uint32_t i = n + threadIdx.x; i < size; i += blockDim.x) sh.list[i] = 0;
+                __syncthreads();
+                block_sort<false>(sh.list, n);
+                const uint32_t each = kListed / blockDim.x, i0 = threadIdx.x * each;
+                uint64_t sum = 0, running;
+                for (uint32_t i = i0; i < min(n, i0 + each); ++i) sum += weigh.of(logit_of(sh.list[i]));
+                block_scan(sum, sh.warp_values, running);
+                running += before;
+                for (uint32_t i = i0; i < min(n, i0 + each); ++i) {
+                    const uint64_t w = weigh.of(logit_of(sh.list[i]));
+                    if (running < wanted && running + w >= wanted) {
+                        for (uint32_t r = 0; r < blocks; ++r) cluster.map_shared_rank(&sh, r)->cut = sh.list[i];
+                    }
+                    running += w;
+                }
+            }
+            cluster.sync();
+            return sh.cut;
+        };
+        if (add && down_to != 0 && down_to - low_before <= kListed) {
+            // ---- many stay, few lie in the bracket: those are put in order ----
+            const float first = (float)low_bin, end = (float)(high_bin + 1);
+            uint64_t above = 0, all_above;
+            gather(cluster, sh, slice, [&](float x, uint32_t) {
+                const float v = place_of(x, high, to_bin, last_bin);
+                if (v < first) above += weigh.of(x);
+                return v >= first && v < end;
+            });
+            tell_parts(cluster, sh, 1, above);
+            cluster.sync();
+            sum_parts(cluster, sh, 1, all_above);
+            cut = rank_list(all_above);
+        } else if (add) {
             // ---- many stay: the bracket by exact weights ----
             for (uint32_t b = threadIdx.x; b < bins; b += blockDim.x) {
                 sh.count[b] = 0;
@@ -807,22 +848,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
                     const float v = place_of(x, high, to_bin, last_bin);
                     return v >= first && v < end && fine_bin(v) == border;
                 });
-                if (rank == 0) {
-                    const uint32_t n = sh.listed;
-                    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) sh.sums[i] = weigh.of(logit_of(sh.list[i]));
-                    __syncthreads();
-                    for (uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-                        const uint64_t c = sh.list[i];
-                        uint64_t over = before;
-#pragma unroll 4
-                        for (uint32_t j = 0; j < n; ++j)
-                            if (sh.list[j] > c) over += sh.sums[j];
-                        if (over < wanted && over + sh.sums[i] >= wanted)
-                            for (uint32_t r = 0; r < blocks; ++r) cluster.map_shared_rank(&sh, r)->cut = c;
-                    }
-                }
-                cluster.sync();
-                cut = sh.cut;
+                cut = rank_list(before);
             } else {
                 cut = find_cut<true>(cluster, sh, slice, weigh, to_bin, bins, 0ull, wanted);
             }
