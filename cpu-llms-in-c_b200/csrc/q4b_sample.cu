@@ -179,7 +179,7 @@ struct Slice {
             }
         }
     }
-    // f over the whole slice, as a block; warp 0 has the head, warp 1 the tail
+    // f over the whole slice, as a block
     template <typename F> __device__ inline void each(F f) const {
         const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 #pragma unroll 1
@@ -268,13 +268,13 @@ __device__ inline uint64_t reach_of(float share, uint64_t total) {
 }
 
 // The elements that `wanted` names, as composites in the list of the cluster's first block; how many there are, or
-// 0xffffffff when they are too many for it.  A block lists its own first: a place in another block's list is a round trip.
+// 0xffffffff when they are too many for it; `bound` is less than any of them, or -infinity.  A block lists its own first: a place in another block's list is a round trip.
 template <typename T, typename F>
-__device__ uint32_t gather(cg::cluster_group &cluster, SampleShared &sh, const Slice<T> &slice, F wanted) {
+__device__ uint32_t gather(cg::cluster_group &cluster, SampleShared &sh, const Slice<T> &slice, float bound, F wanted) {
     if (threadIdx.x == 0) sh.own_listed = 0;
     __syncthreads();
     slice.each([&](float x, uint32_t i) {
-        if (wanted(x, i)) {
+        if (!(x < bound) && wanted(x, i)) {  // one comparison for most
             const uint32_t place = atomicAdd(&sh.own_listed, 1u);
             if (place < kListed) sh.sums[place] = composite(x, slice.begin + i);
         }
@@ -350,7 +350,7 @@ __device__ __noinline__ uint64_t find_cut(cg::cluster_group &cluster, SampleShar
         before = sh.found_before;
         if (border_count <= kListed) {
             // gather the bin in the first block and rank it there
-            gather(cluster, sh, slice, [&](float x, uint32_t i) {
+            gather(cluster, sh, slice, -INFINITY, [&](float x, uint32_t i) {
                 const uint64_t c = composite(x, slice.begin + i);
                 return in_span(c) && bin_of(x, c) == border;
             });
@@ -423,6 +423,31 @@ __device__ void block_sort(V *values, uint32_t n) {
     }
 }
 
+// The same for at most an element per thread, which gets the one of its place: by exchanges within the warps as far as
+// those reach.  `size` is the power of two that values[0, size) is filled to.
+__device__ inline uint64_t thread_sort(uint64_t *values, uint32_t size) {
+    const uint32_t i = threadIdx.x;
+    uint64_t own = i < size ? values[i] : 0;
+#pragma unroll 1
+    for (uint32_t k = 2; k <= size; k *= 2) {
+#pragma unroll 1
+        for (uint32_t j = k / 2; j > 0; j /= 2) {
+            uint64_t other;
+            if (j >= 32) {
+                __syncthreads();
+                values[i] = own;
+                __syncthreads();
+                other = values[i ^ j];
+            } else {
+                other = __shfl_xor_sync(0xffffffffu, own, j);
+            }
+            const bool larger = ((i & j) == 0) == ((i & k) == 0);
+            own = (own > other) == larger ? own : other;
+        }
+    }
+    return own;
+}
+
 __device__ inline uint64_t target_of(float uniform, uint64_t total) {
     const double aim = uniform > 0.0f ? floor((double)uniform * (double)total) : 0.0;
     const uint64_t target = aim < (double)total ? (uint64_t)aim : total - 1;
@@ -441,26 +466,8 @@ __device__ __noinline__ void finish_list(const SampleArgs &p, uint32_t row, Samp
     if (n > blockDim.x) block_sort<false>(sh.list, n);
     const uint32_t first = k != 0 && k < n ? k : n;
     if (n <= blockDim.x) {
-        // an element per thread, sorted by exchanges within the warps as far as those reach
         const uint32_t i = threadIdx.x;
-        uint64_t own = i < size ? sh.list[i] : 0;
-#pragma unroll 1
-        for (uint32_t k2 = 2; k2 <= size; k2 *= 2) {
-#pragma unroll 1
-            for (uint32_t j = k2 / 2; j > 0; j /= 2) {
-                uint64_t other;
-                if (j >= 32) {
-                    __syncthreads();
-                    sh.list[i] = own;
-                    __syncthreads();
-                    other = sh.list[i ^ j];
-                } else {
-                    other = __shfl_xor_sync(0xffffffffu, own, j);
-                }
-                const bool larger = ((i & j) == 0) == ((i & k2) == 0);
-                own = (own > other) == larger ? own : other;
-            }
-        }
+        const uint64_t own = thread_sort(sh.list, size);
         const uint64_t weight = i < n ? weigh.of(logit_of(own)) : 0;
         uint64_t above;
         const uint64_t sum_first = block_scan(i < first ? weight : 0, sh.warp_values, above);
@@ -662,6 +669,13 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     // the least weight that stays, in units (a NaN is none)
     const uint64_t least = floor_p > 0.0f ? (uint64_t)ceil((double)fminf(floor_p, 1.0f) * (double)kOne) : 0;
 
+    // less than every value whose place is below `end`: the place's roundings and the value's own are 2^-22 of them
+    auto value_below = [&](float end) {
+        if (end > last_bin) return -INFINITY;
+        if (high == INFINITY) return high;
+        return high - end / to_bin * 1.000001f - fabsf(high) * 1e-6f;
+    };
+
     uint64_t cut = 0;
     if (k != 0 && k <= kListed / 2) {
         // ---- few by count ----
@@ -684,7 +698,8 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         cluster.sync();
         if (sh.found_count != 0) {  // fewer threads than k otherwise
             const float end = (float)(sh.high_bin + 1);
-            if (gather(cluster, sh, slice, [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; }) <= kListed) {
+            if (gather(cluster, sh, slice, value_below(end), [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; }) <=
+                kListed) {
                 if (rank == 0) finish_list(p, row, sh, weigh, k, share, 0, least, uniform);
                 return;
             }
@@ -760,7 +775,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         if (down_to != 0 && down_to <= kListed) {
             // ---- few stay ----
             const float end = (float)(high_bin + 1);
-            gather(cluster, sh, slice, [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; });
+            gather(cluster, sh, slice, value_below(end), [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; });
             if (rank == 0) finish_list(p, row, sh, weigh, k, share, everything, least, uniform);
             return;
         }
@@ -772,8 +787,15 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
                 while (size < n) size *= 2;
                 for (uint32_t i = n + threadIdx.x; i < size; i += blockDim.x) sh.list[i] = 0;
                 __syncthreads();
-                block_sort<false>(sh.list, n);
-                const uint32_t each = kListed / blockDim.x, i0 = threadIdx.x * each;
+                if (n <= blockDim.x) {
+                    const uint64_t own = thread_sort(sh.list, size);
+                    __syncthreads();
+                    sh.list[threadIdx.x] = own;
+                    __syncthreads();
+                } else {
+                    block_sort<false>(sh.list, n);
+                }
+                const uint32_t each = n <= blockDim.x ? 1 : kListed / blockDim.x, i0 = threadIdx.x * each;
                 uint64_t sum = 0, running;
                 for (uint32_t i = i0; i < min(n, i0 + each); ++i) sum += weigh.of(logit_of(sh.list[i]));
                 block_scan(sum, sh.warp_values, running);
@@ -793,7 +815,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             // ---- many stay, few lie in the bracket: those are put in order ----
             const float first = (float)low_bin, end = (float)(high_bin + 1);
             uint64_t above = 0, all_above;
-            gather(cluster, sh, slice, [&](float x, uint32_t) {
+            gather(cluster, sh, slice, value_below(end), [&](float x, uint32_t) {
                 const float v = place_of(x, high, to_bin, last_bin);
                 if (v < first) above += weigh.of(x);
                 return v >= first && v < end;
@@ -844,7 +866,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             const uint32_t border = sh.fine_bin, border_count = sh.fine_count;
             const uint64_t before = sh.found_before;
             if (border_count != 0 && border_count <= kListed) {
-                gather(cluster, sh, slice, [&](float x, uint32_t) {
+                gather(cluster, sh, slice, value_below(end), [&](float x, uint32_t) {
                     const float v = place_of(x, high, to_bin, last_bin);
                     return v >= first && v < end && fine_bin(v) == border;
                 });
