@@ -146,7 +146,9 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
     // [query rows][rings of the warps]; the rings' place is also where the warps' sums meet
     T *const query = reinterpret_cast<T *>(smem);
     uint8_t *const rings = smem + kRows * D * 2;
-    float *const sums = reinterpret_cast<float *>(rings);             // [warps][kRows][D]
+    // [warps][kRows][D], rows four floats further apart: a warp's stores then fall into 32 different banks
+    constexpr uint32_t kSumRow = D + 4;
+    float *const sums = reinterpret_cast<float *>(rings);
     __shared__ float top_of[kWarps][kRows], total_of[kWarps][kRows];
     __shared__ uint64_t scan[kWarps];
     __shared__ uint64_t found_before;
@@ -156,47 +158,72 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
     const uint32_t ring = smem_u32(rings) + warp * kItem * kItems;
 
     // ---- this thread block's range of the list of groups ----
-    uint64_t all = 0, before;
-    for (uint32_t s0 = 0; s0 < p.batch.sequences; s0 += kThreads) {
-        const uint32_t s = s0 + threadIdx.x;
-        uint64_t mine = 0;
-        if (s < p.batch.sequences)
-            mine = sequence_groups(p, sequence_rows(p.batch, p.cache.page_tokens, s, p.status), kRows);
-        all += block_scan(mine, scan, before);
-    }
-    const uint64_t share = max((all + gridDim.x - 1) / gridDim.x, (uint64_t)kLeastShare);
-    const uint64_t begin = (uint64_t)blockIdx.x * share, end = min(begin + share, all);
-    if (begin >= end) return;
-    for (uint64_t s0 = 0, sum = 0; sum <= begin; s0 += kThreads) {
-        const uint32_t s = (uint32_t)s0 + threadIdx.x;
-        uint64_t mine = 0;
-        if (s < p.batch.sequences)
-            mine = sequence_groups(p, sequence_rows(p.batch, p.cache.page_tokens, s, p.status), kRows);
-        const uint64_t total = block_scan(mine, scan, before);
-        if (sum + before <= begin && begin < sum + before + mine) {
-            found_sequence = s;
-            found_before = sum + before;
-        }
-        sum += total;
-    }
-    __syncthreads();
     UnitWalk u;
     u.chunk_rows = kRows;
-    u.sequence = found_sequence;
-    u.rows = sequence_rows(p.batch, p.cache.page_tokens, u.sequence, p.status);
-    u.chunks = ceil_div(u.rows.count * p.group, kRows);
     u.head = 0;
     u.chunk = 0;
-    uint64_t unit_begin = found_before;
-    unit_groups(p, u);
-    // the unit within the sequence: heads outside, chunks of rows inside
-    while (unit_begin + u.groups.count() <= begin) {
-        unit_begin += u.groups.count();
-        if (++u.chunk == u.chunks) {
-            u.chunk = 0;
-            ++u.head;
+    uint64_t begin, end, share, unit_begin;  // in groups; a thread block has [begin, end), `share` of them at most
+    uint64_t unit_stride = 0;                // not 0: units begin this far apart, each cut into whole shares
+    if (p.batch.sequences == 1) {
+        // One sequence: its key heads are equally long, and cut into equally many shares each no thread block meets the
+        // end of one and the start of the next.
+        u.sequence = 0;
+        u.rows = sequence_rows(p.batch, p.cache.page_tokens, 0, p.status);
+        u.chunks = ceil_div(u.rows.count * p.group, kRows);
+        if (u.chunks == 0) return;
+        if (u.chunks == 1 && p.cache.kv_heads <= gridDim.x) {
+            unit_groups(p, u);
+            const uint32_t count = u.groups.count();
+            const uint32_t parts = min(gridDim.x / p.cache.kv_heads, ceil_div(count, kLeastShare));
+            share = ceil_div(count, parts);
+            unit_stride = share * parts;
+            u.head = blockIdx.x / parts;
+            if (u.head >= p.cache.kv_heads) return;
+            unit_begin = u.head * unit_stride;
+            begin = unit_begin + blockIdx.x % parts * share;
+            end = min(begin + share, unit_begin + count);
+            if (begin >= end) return;
         }
+    }
+    if (unit_stride == 0) {
+        uint64_t all = 0, before, mine = 0;
+        for (uint32_t s0 = 0; s0 < p.batch.sequences; s0 += kThreads) {
+            const uint32_t s = s0 + threadIdx.x;
+            mine = s < p.batch.sequences ? sequence_groups(p, sequence_rows(p.batch, p.cache.page_tokens, s, p.status), kRows) : 0;
+            all += block_scan(mine, scan, before);
+        }
+        share = max((all + gridDim.x - 1) / gridDim.x, (uint64_t)kLeastShare);
+        begin = (uint64_t)blockIdx.x * share;
+        end = min(begin + share, all);
+        if (begin >= end) return;
+        for (uint64_t s0 = 0, sum = 0; sum <= begin; s0 += kThreads) {
+            const uint32_t s = (uint32_t)s0 + threadIdx.x;
+            uint64_t total = all;  // a batch of one round has its numbers at hand
+            if (p.batch.sequences > kThreads) {
+                mine = s < p.batch.sequences ? sequence_groups(p, sequence_rows(p.batch, p.cache.page_tokens, s, p.status), kRows) : 0;
+                total = block_scan(mine, scan, before);
+            }
+            if (sum + before <= begin && begin < sum + before + mine) {
+                found_sequence = s;
+                found_before = sum + before;
+            }
+            sum += total;
+        }
+        __syncthreads();
+        u.sequence = found_sequence;
+        u.rows = sequence_rows(p.batch, p.cache.page_tokens, u.sequence, p.status);
+        u.chunks = ceil_div(u.rows.count * p.group, kRows);
+        unit_begin = found_before;
         unit_groups(p, u);
+        // the unit within the sequence: heads outside, chunks of rows inside
+        while (unit_begin + u.groups.count() <= begin) {
+            unit_begin += u.groups.count();
+            if (++u.chunk == u.chunks) {
+                u.chunk = 0;
+                ++u.head;
+            }
+            unit_groups(p, u);
+        }
     }
 
     const float scale = p.scale * 1.44269504088896341f;
@@ -210,21 +237,7 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
         const uint32_t keys_end = u.groups.end == 0 ? 0 : u.rows.length;
         const uint32_t *table = p.batch.table + (size_t)u.sequence * p.batch.table_stride;
 
-        // ---- query rows, pieces of a row turned by the row (no bank conflicts for ldmatrix) ----
-        __syncthreads();
-        for (uint32_t i = threadIdx.x; i < kRows * kChunks; i += kThreads) {
-            const uint32_t row = i / kChunks, piece = i % kChunks;
-            uint4 value = make_uint4(0, 0, 0, 0);
-            if (row < unit_rows) {
-                const uint32_t flat = unit_row0 + row;
-                const T *from = static_cast<const T *>(p.q) + (size_t)(u.rows.begin + flat / p.group) * p.ldq +
-                                (size_t)(u.head * p.group + flat % p.group) * D + piece * 8;
-                value = *reinterpret_cast<const uint4 *>(from);
-            }
-            *reinterpret_cast<uint4 *>(query + row * D + ((piece ^ (row & 7)) * 8)) = value;
-        }
-        __syncthreads();
-
+        __syncthreads();  // the last unit's sums have been read: the rings are free
         // the places of this lane's rows 8 r + 2 t and 8 r + 2 t + 1 (negative: a row that sees nothing)
         int64_t place[R][2];
 #pragma unroll
@@ -283,6 +296,20 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
         };
 #pragma unroll
         for (uint32_t i = 0; i + 1 < kItems; ++i) fetch(i);
+
+        // ---- query rows, pieces of a row turned by the row (no bank conflicts for ldmatrix) ----
+        for (uint32_t i = threadIdx.x; i < kRows * kChunks; i += kThreads) {
+            const uint32_t row = i / kChunks, piece = i % kChunks;
+            uint4 value = make_uint4(0, 0, 0, 0);
+            if (row < unit_rows) {
+                const uint32_t flat = unit_row0 + row;
+                const T *from = static_cast<const T *>(p.q) + (size_t)(u.rows.begin + flat / p.group) * p.ldq +
+                                (size_t)(u.head * p.group + flat % p.group) * D + piece * 8;
+                value = *reinterpret_cast<const uint4 *>(from);
+            }
+            *reinterpret_cast<uint4 *>(query + row * D + ((piece ^ (row & 7)) * 8)) = value;
+        }
+        __syncthreads();
 
         const uint32_t q_base = smem_u32(query);
         for (uint32_t index = 0; index < my_groups; ++index) {
@@ -436,7 +463,7 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
                 for (uint32_t w = 1; w < kWarps; ++w) high = fmaxf(high, top_of[w][row]);
                 const float factor = top[r][i] == -INFINITY ? 0.0f : exp2_fast(top[r][i] - high);
                 // a warp that saw nothing has sums of zero (and NaN only from rows that see a NaN)
-                float *to = sums + ((size_t)warp * kRows + row) * D + gid;
+                float *to = sums + (warp * kRows + row) * kSumRow + gid;
 #pragma unroll
                 for (int m = 0; m < D / 16; ++m) {
                     to[16 * m] = out[r][m][i] * factor;
@@ -447,8 +474,8 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
         __syncthreads();
         // the unit's first thread block has its counter; a thread block leaves two sums at most: of the unit that it
         // begins in the middle of, and of the one that it does not finish
-        const uint32_t first_block = (uint32_t)(unit_begin / share);
-        const uint32_t last_block = (uint32_t)((unit_end - 1) / share);
+        const uint32_t first_block = whole ? 0 : (uint32_t)(unit_begin / share);
+        const uint32_t last_block = whole ? 0 : (uint32_t)((unit_end - 1) / share);
         const uint32_t slot = 2 * blockIdx.x + (unit_begin < begin ? 0u : 1u);
         constexpr uint32_t kSlotFloats = kMostRows * (kMostHead + 2);
         float *const partial = p.partials + (size_t)slot * kSlotFloats;  // [rows][D], then maxima, then totals
@@ -460,7 +487,7 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
             for (uint32_t w = 0; w < kWarps; ++w) high = fmaxf(high, top_of[w][row]);
 #pragma unroll
             for (uint32_t w = 0; w < kWarps; ++w) {
-                const float4 part = *reinterpret_cast<const float4 *>(sums + ((size_t)w * kRows + row) * D + column);
+                const float4 part = *reinterpret_cast<const float4 *>(sums + (w * kRows + row) * kSumRow + column);
                 sum.x += part.x; sum.y += part.y; sum.z += part.z; sum.w += part.w;
                 mass += top_of[w][row] == -INFINITY ? total_of[w][row] : total_of[w][row] * exp2_fast(top_of[w][row] - high);
             }
@@ -489,25 +516,54 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
             __syncthreads();
             if (last_to_arrive) {
                 __threadfence();
+                // the first block's sum is of the unit that it does not finish, the others' of the one they begin in
+                const uint32_t parts = last_block - first_block + 1;
+                const float *const from = p.partials + (size_t)(2 * first_block) * kSlotFloats;
+                auto slot_of = [&](uint32_t part) { return from + (size_t)(2 * part + (part == 0 ? 1u : 0u)) * kSlotFloats; };
+                float *const factor_of = sums;                          // [parts][kRows], in the rings' place
+                float *const mass_of = sums + (size_t)gridDim.x * kRows;
+                for (uint32_t i = threadIdx.x; i < parts * unit_rows; i += kThreads) {
+                    const uint32_t part = i / unit_rows, row = i % unit_rows;
+                    factor_of[part * kRows + row] = __ldcg(slot_of(part) + kMostRows * kMostHead + row);
+                    mass_of[part * kRows + row] = __ldcg(slot_of(part) + kMostRows * (kMostHead + 1) + row);
+                }
+                __syncthreads();
+                for (uint32_t row = warp; row < unit_rows; row += kWarps) {
+                    float high = -INFINITY, mass = 0.0f;
+                    for (uint32_t part = lane; part < parts; part += 32) high = fmaxf(high, factor_of[part * kRows + row]);
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, d));
+                    for (uint32_t part = lane; part < parts; part += 32) {
+                        const float own = factor_of[part * kRows + row];
+                        const float factor = own == -INFINITY ? 1.0f : exp2_fast(own - high);
+                        factor_of[part * kRows + row] = factor;
+                        mass += mass_of[part * kRows + row] * factor;
+                    }
+#pragma unroll
+                    for (int d = 16; d > 0; d >>= 1) mass += __shfl_xor_sync(0xffffffffu, mass, d);
+                    if (lane == 0) total_of[0][row] = mass;
+                }
+                __syncthreads();
                 for (uint32_t i = threadIdx.x; i < unit_rows * (D / 4); i += kThreads) {
                     const uint32_t row = i / (D / 4), column = (i % (D / 4)) * 4;
-                    // the first block's sum is of the unit that it does not finish, the others' of the one they begin in
-                    float high = -INFINITY;
-                    for (uint32_t b = first_block; b <= last_block; ++b)
-                        high = fmaxf(high, __ldcg(p.partials + (size_t)(2 * b + (b == first_block ? 1 : 0)) * kSlotFloats +
-                                                  kMostRows * kMostHead + row));
                     float4 sum = make_float4(0, 0, 0, 0);
-                    float mass = 0.0f;
-#pragma unroll 4
-                    for (uint32_t b = first_block; b <= last_block; ++b) {
-                        const float *from = p.partials + (size_t)(2 * b + (b == first_block ? 1 : 0)) * kSlotFloats;
-                        const float own = __ldcg(from + kMostRows * kMostHead + row);
-                        const float factor = own == -INFINITY ? 1.0f : exp2_fast(own - high);
-                        const float4 part = __ldcg(reinterpret_cast<const float4 *>(from + row * D + column));
-                        sum.x += part.x * factor; sum.y += part.y * factor;
-                        sum.z += part.z * factor; sum.w += part.w * factor;
-                        mass += __ldcg(from + kMostRows * (kMostHead + 1) + row) * factor;
+                    // sixteen loads on their way per thread: one thread block takes in 60 bytes per clock like that
+                    for (uint32_t part0 = 0; part0 < parts; part0 += 16) {
+                        float4 piece[16];
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e)
+                            if (part0 + e < parts)
+                                piece[e] = __ldcg(reinterpret_cast<const float4 *>(slot_of(part0 + e) + row * D + column));
+#pragma unroll
+                        for (uint32_t e = 0; e < 16; ++e) {
+                            if (part0 + e < parts) {
+                                const float factor = factor_of[(part0 + e) * kRows + row];
+                                sum.x += piece[e].x * factor; sum.y += piece[e].y * factor;
+                                sum.z += piece[e].z * factor; sum.w += piece[e].w * factor;
+                            }
+                        }
                     }
+                    const float mass = total_of[0][row];
                     const uint32_t flat = unit_row0 + row;
                     T *to = static_cast<T *>(p.out) + (size_t)(u.rows.begin + flat / p.group) * p.ldo +
                             (size_t)(u.head * p.group + flat % p.group) * D + column;
@@ -539,7 +595,7 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
 
 template <typename T, int D, int R>
 cudaError_t launch_instance(const AttentionArgs &args, int sm_count, cudaStream_t stream) {
-    const size_t stream_bytes = (size_t)kWarps * Ring<D>::item * Ring<D>::items, sum_bytes = (size_t)kWarps * 8 * R * D * 4;
+    const size_t stream_bytes = (size_t)kWarps * Ring<D>::item * Ring<D>::items, sum_bytes = (size_t)kWarps * 8 * R * (D + 4) * 4;
     const size_t smem = (size_t)8 * R * D * 2 + (stream_bytes > sum_bytes ? stream_bytes : sum_bytes);
     static bool configured[kMaxDevices] = {};
     const int slot = device_slot();
