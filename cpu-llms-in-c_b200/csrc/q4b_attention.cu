@@ -20,12 +20,15 @@
 // the workspace; whoever arrives last adds them up in block order, so results do not depend on timing.
 #include "q4b_cache.cuh"
 
+#include <cooperative_groups.h>
 #include <cmath>
 #include <type_traits>
 
 namespace q4b {
 
 namespace {
+
+namespace cg = cooperative_groups;
 
 constexpr uint32_t kWarps = 8;
 constexpr uint32_t kThreads = kWarps * 32;
@@ -36,6 +39,7 @@ constexpr uint32_t kBlocksPerSm = 1;
 // a unit's share of a thread block is at least this many groups (one per warp): fewer would leave warps idle while
 // adding sums to join
 constexpr uint32_t kLeastShare = 8;
+constexpr uint32_t kCluster = 8;        // thread blocks of a cluster, where one sequence has the GPU to itself
 
 template <int D> struct Ring {
     static constexpr uint32_t item = kKeys * D * 2;               // 16 keys or values
@@ -136,7 +140,8 @@ __device__ inline uint64_t block_scan(uint64_t value, uint64_t *scratch, uint64_
     return total;
 }
 
-template <typename T, int D, int R>
+// CLUSTER: launched in clusters of kCluster, for one sequence
+template <typename T, int D, int R, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 attend_kernel(const __grid_constant__ AttentionArgs p) {
     constexpr uint32_t kRows = 8 * R;
@@ -163,26 +168,27 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
     u.head = 0;
     u.chunk = 0;
     uint64_t begin, end, share, unit_begin;  // in groups; a thread block has [begin, end), `share` of them at most
-    uint64_t unit_stride = 0;                // not 0: units begin this far apart, each cut into whole shares
-    if (p.batch.sequences == 1) {
-        // One sequence: its key heads are equally long, and cut into equally many shares each no thread block meets the
-        // end of one and the start of the next.
+    uint64_t unit_stride = 0;                // not 0: units begin this far apart, each cut into whole clusters of shares
+    uint32_t unit_clusters = 0;              // clusters that share a unit
+    if constexpr (CLUSTER) {
+        // One sequence: its key heads are equally long.  Each is cut into equally many shares, a whole number of clusters,
+        // so the shares' sums meet in distributed shared memory and few or none go through the workspace.
         u.sequence = 0;
         u.rows = sequence_rows(p.batch, p.cache.page_tokens, 0, p.status);
         u.chunks = ceil_div(u.rows.count * p.group, kRows);
-        if (u.chunks == 0) return;
-        if (u.chunks == 1 && p.cache.kv_heads <= gridDim.x) {
+        const uint32_t clusters = gridDim.x / kCluster;
+        if (u.chunks == 1 && p.cache.kv_heads <= clusters) {
             unit_groups(p, u);
             const uint32_t count = u.groups.count();
-            const uint32_t parts = min(gridDim.x / p.cache.kv_heads, ceil_div(count, kLeastShare));
+            unit_clusters = min(clusters / p.cache.kv_heads, ceil_div(count, kCluster * kLeastShare));
+            const uint32_t parts = unit_clusters * kCluster;
             share = ceil_div(count, parts);
             unit_stride = share * parts;
             u.head = blockIdx.x / parts;
             if (u.head >= p.cache.kv_heads) return;
             unit_begin = u.head * unit_stride;
-            begin = unit_begin + blockIdx.x % parts * share;
+            begin = unit_begin + min(blockIdx.x % parts * (uint32_t)share, count);  // the last shares may be empty
             end = min(begin + share, unit_begin + count);
-            if (begin >= end) return;
         }
     }
     if (unit_stride == 0) {
@@ -227,7 +233,8 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
     }
 
     const float scale = p.scale * 1.44269504088896341f;
-    for (uint64_t position = begin; position < end;) {
+    uint64_t position = begin;
+    do {
         const uint32_t unit_count = u.groups.count();
         const uint64_t unit_end = unit_begin + unit_count;
         const uint32_t g0 = (uint32_t)(position - unit_begin), g1 = (uint32_t)(min(unit_end, end) - unit_begin);
@@ -472,6 +479,120 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
             }
         }
         __syncthreads();
+        if (CLUSTER && unit_stride != 0) {
+            cg::cluster_group cluster = cg::this_cluster();
+            const uint32_t rank = cluster.block_rank(), items = unit_rows * (D / 4);
+            float *const own_sum = sums + kWarps * kRows * kSumRow, *const own_top = own_sum + kRows * D,
+                        *const own_total = own_top + kRows;
+            for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
+                const uint32_t row = i / (D / 4), column = (i % (D / 4)) * 4;
+                float4 sum = make_float4(0, 0, 0, 0);
+                float high = -INFINITY, mass = 0.0f;
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; ++w) high = fmaxf(high, top_of[w][row]);
+#pragma unroll
+                for (uint32_t w = 0; w < kWarps; ++w) {
+                    const float4 part = *reinterpret_cast<const float4 *>(sums + (w * kRows + row) * kSumRow + column);
+                    sum.x += part.x; sum.y += part.y; sum.z += part.z; sum.w += part.w;
+                    mass += top_of[w][row] == -INFINITY ? total_of[w][row] : total_of[w][row] * exp2_fast(top_of[w][row] - high);
+                }
+                *reinterpret_cast<float4 *>(own_sum + row * D + column) = sum;
+                if (column == 0) {
+                    own_top[row] = high;
+                    own_total[row] = mass;
+                }
+            }
+            cluster.sync();
+            // every block adds an eighth of the outputs up over the cluster
+            const uint32_t each = (items + kCluster - 1) / kCluster, i = rank * each + threadIdx.x;
+            const bool mine = threadIdx.x < each && i < items;
+            const uint32_t row = mine ? i / (D / 4) : 0, column = (i % (D / 4)) * 4;
+            float4 sum = make_float4(0, 0, 0, 0);
+            float high = -INFINITY, mass = 0.0f;
+            if (mine) {
+                float top_r[kCluster], total_r[kCluster];
+                float4 sum_r[kCluster];
+#pragma unroll
+                for (uint32_t r = 0; r < kCluster; ++r) {
+                    top_r[r] = cluster.map_shared_rank(own_top, r)[row];
+                    total_r[r] = cluster.map_shared_rank(own_total, r)[row];
+                    sum_r[r] = *reinterpret_cast<const float4 *>(cluster.map_shared_rank(own_sum, r) + row * D + column);
+                    high = fmaxf(high, top_r[r]);
+                }
+#pragma unroll
+                for (uint32_t r = 0; r < kCluster; ++r) {
+                    const float factor = top_r[r] == -INFINITY ? 1.0f : exp2_fast(top_r[r] - high);
+                    sum.x += sum_r[r].x * factor; sum.y += sum_r[r].y * factor;
+                    sum.z += sum_r[r].z * factor; sum.w += sum_r[r].w * factor;
+                    mass += total_r[r] * factor;
+                }
+            }
+            auto answer = [&](const float4 &value, float total) {
+                const uint32_t flat = unit_row0 + row;
+                T *to = static_cast<T *>(p.out) + (size_t)(u.rows.begin + flat / p.group) * p.ldo +
+                        (size_t)(u.head * p.group + flat % p.group) * D + column;
+                const float over = total == 0.0f ? 0.0f : 1.0f / total;
+                *reinterpret_cast<uint2 *>(to) = make_uint2(pack<T>(value.x * over, value.y * over), pack<T>(value.z * over, value.w * over));
+            };
+            auto arrived = cluster.barrier_arrive();  // this block has read the others' sums
+            if (unit_clusters == 1) {
+                if (mine) answer(sum, mass);
+            } else {
+                // blocks of equal rank in the unit's clusters have the same outputs: the last of them adds up in cluster order
+                constexpr uint32_t kItems4 = kMostRows * kMostHead / 4, kSlot = kItems4 * 6;  // sums, then (top, total) pairs
+                float *const unit_slots = p.partials + (size_t)(u.head * unit_clusters) * kSlot;
+                const uint32_t slot = blockIdx.x / kCluster % unit_clusters;
+                if (mine) {
+                    reinterpret_cast<float4 *>(unit_slots + (size_t)slot * kSlot)[i] = sum;
+                    reinterpret_cast<float2 *>(unit_slots + (size_t)slot * kSlot + 4 * kItems4)[i] = make_float2(high, mass);
+                }
+                __threadfence();
+                __syncthreads();
+                if (threadIdx.x == 0) {
+                    uint32_t *const counter = p.arrivals + u.head * kCluster + rank;
+                    last_to_arrive = atomicAdd(counter, 1u) == unit_clusters - 1 ? 1u : 0u;
+                    if (last_to_arrive) *counter = 0;
+                }
+                __syncthreads();
+                if (last_to_arrive && mine) {
+                    __threadfence();
+                    high = -INFINITY;
+                    mass = 0.0f;
+                    sum = make_float4(0, 0, 0, 0);
+                    for (uint32_t c0 = 0; c0 < unit_clusters; c0 += 8) {
+                        float4 piece[8];
+                        float2 told[8];
+                        float grown = high;
+#pragma unroll
+                        for (uint32_t e = 0; e < 8; ++e) {
+                            told[e] = make_float2(-INFINITY, 0.0f);
+                            piece[e] = make_float4(0, 0, 0, 0);
+                            if (c0 + e < unit_clusters) {
+                                const float *const from = unit_slots + (size_t)(c0 + e) * kSlot;
+                                piece[e] = __ldcg(reinterpret_cast<const float4 *>(from) + i);
+                                told[e] = __ldcg(reinterpret_cast<const float2 *>(from + 4 * kItems4) + i);
+                            }
+                        }
+#pragma unroll
+                        for (uint32_t e = 0; e < 8; ++e) grown = fmaxf(grown, told[e].x);
+                        const float keep = high == -INFINITY ? 1.0f : exp2_fast(high - grown);
+                        sum.x *= keep; sum.y *= keep; sum.z *= keep; sum.w *= keep;
+                        mass *= keep;
+                        high = grown;
+#pragma unroll
+                        for (uint32_t e = 0; e < 8; ++e) {
+                            const float factor = told[e].x == -INFINITY ? 1.0f : exp2_fast(told[e].x - high);
+                            sum.x += piece[e].x * factor; sum.y += piece[e].y * factor;
+                            sum.z += piece[e].z * factor; sum.w += piece[e].w * factor;
+                            mass += told[e].y * factor;
+                        }
+                    }
+                    answer(sum, mass);
+                }
+            }
+            cluster.barrier_wait(static_cast<cg::cluster_group::arrival_token &&>(arrived));
+            return;
+        }
         // the unit's first thread block has its counter; a thread block leaves two sums at most: of the unit that it
         // begins in the middle of, and of the one that it does not finish
         const uint32_t first_block = whole ? 0 : (uint32_t)(unit_begin / share);
@@ -590,28 +711,51 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
             }
             unit_groups(p, u);
         }
-    }
+    } while (position < end);
 }
 
-template <typename T, int D, int R>
+template <typename T, int D, int R, bool CLUSTER>
 cudaError_t launch_instance(const AttentionArgs &args, int sm_count, cudaStream_t stream) {
-    const size_t stream_bytes = (size_t)kWarps * Ring<D>::item * Ring<D>::items, sum_bytes = (size_t)kWarps * 8 * R * (D + 4) * 4;
-    const size_t smem = (size_t)8 * R * D * 2 + (stream_bytes > sum_bytes ? stream_bytes : sum_bytes);
-    static bool configured[kMaxDevices] = {};
+    constexpr size_t stream_bytes = (size_t)kWarps * Ring<D>::item * Ring<D>::items;
+    constexpr size_t sum_bytes = (size_t)kWarps * 8 * R * (D + 4) * 4 + (size_t)8 * R * (D + 2) * 4;
+    constexpr size_t smem = (size_t)8 * R * D * 2 + (stream_bytes > sum_bytes ? stream_bytes : sum_bytes);
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3((unsigned)sm_count * kBlocksPerSm / (CLUSTER ? kCluster : 1) * (CLUSTER ? kCluster : 1));
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = kCluster;
+    attribute[0].val.clusterDim.y = 1;
+    attribute[0].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = CLUSTER ? 1 : 0;
+    static int room[kMaxDevices] = {};  // clusters that a device holds at once; 1 where there are none
     const int slot = device_slot();
-    if (slot < 0 || !configured[slot]) {
-        cudaError_t status = cudaFuncSetAttribute(attend_kernel<T, D, R>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    int clusters = slot >= 0 ? room[slot] : 0;
+    if (clusters == 0) {
+        cudaError_t status = cudaFuncSetAttribute(attend_kernel<T, D, R, CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
         if (status != cudaSuccess) return status;
-        if (slot >= 0) configured[slot] = true;
+        clusters = 1;
+        if (CLUSTER) {
+            status = cudaOccupancyMaxActiveClusters(&clusters, attend_kernel<T, D, R, CLUSTER>, &config);
+            if (status != cudaSuccess) return status;
+            if (clusters < 1) clusters = 1;
+            if (clusters > sm_count / (int)kCluster) clusters = sm_count / (int)kCluster;
+        }
+        if (slot >= 0) room[slot] = clusters;
     }
-    attend_kernel<T, D, R><<<(unsigned)sm_count * kBlocksPerSm, kThreads, smem, stream>>>(args);
-    return cudaGetLastError();
+    if (CLUSTER) config.gridDim = dim3((unsigned)clusters * kCluster);
+    return cudaLaunchKernelEx(&config, attend_kernel<T, D, R, CLUSTER>, args);
 }
 
 template <typename T, int D>
 cudaError_t launch_rows(const AttentionArgs &args, int sm_count, cudaStream_t stream) {
     const uint64_t rows = (uint64_t)(args.most_tokens != 0 ? args.most_tokens : args.batch.tokens) * args.group;
-    return rows <= 8 ? launch_instance<T, D, 1>(args, sm_count, stream) : launch_instance<T, D, 2>(args, sm_count, stream);
+    if (args.batch.sequences == 1)
+        return rows <= 8 ? launch_instance<T, D, 1, true>(args, sm_count, stream) : launch_instance<T, D, 2, true>(args, sm_count, stream);
+    return rows <= 8 ? launch_instance<T, D, 1, false>(args, sm_count, stream) : launch_instance<T, D, 2, false>(args, sm_count, stream);
 }
 
 template <typename T>
