@@ -111,6 +111,18 @@ def test_growing_scores(q4b, ctx):
             assert (np.abs(got - want) <= tolerance).all()
 
 
+@pytest.mark.parametrize("dtype,head,page,kv_heads,group,new,length,window,sinks", [
+    ("f16", 256, 16, 4, 6, 1, 1, 0, 0), ("f16", 256, 16, 4, 6, 1, 130, 0, 0), ("bf16", 256, 64, 4, 6, 1, 9001, 0, 0),
+    ("f16", 128, 32, 1, 4, 1, 20011, 0, 0), ("bf16", 64, 16, 2, 8, 2, 5000, 0, 0), ("f16", 128, 16, 3, 3, 5, 3001, 777, 20),
+    ("bf16", 256, 16, 1, 1, 16, 40, 0, 0), ("f16", 64, 64, 24, 1, 1, 700, 0, 0), ("f16", 64, 16, 1, 16, 1, 4097, 4000, 3)])
+def test_one_sequence(q4b, ctx, dtype, head, page, kv_heads, group, new, length, window, sinks):
+    """Its heads are cut into shares that meet in clusters, and those in the workspace -- or not, with many heads."""
+    rng = np.random.default_rng(length)
+    batch = Batch(rng, [new], [length], page, kv_heads, head, dtype, pad=1)
+    check(q4b, ctx, batch, kv_heads * group, window, sinks)
+    check(q4b, ctx, batch, kv_heads * group, window, sinks, most_tokens=1)   # a hint that is too small
+
+
 def test_many_unlike_sequences(q4b, ctx):
     rng = np.random.default_rng(5)
     lengths = rng.integers(1, 90, size=300)
