@@ -82,9 +82,14 @@ struct Unit {
     uint32_t first, size;                  // this thread block's share of them
     int64_t least, most, place0;           // places of the first and the last row; of the sequence's first new token
     __device__ inline uint32_t key(uint32_t j) const { return tiles.at(first + j) * kTileKeys; }
-    __device__ inline bool clear(const AttentionArgs &a, uint32_t key0) const {
-        return (int64_t)key0 + kTileKeys - 1 <= least &&
-               (a.window == 0 || (int64_t)key0 > most - (int64_t)a.window || (uint64_t)key0 + kTileKeys <= a.sinks);
+    __device__ inline bool clear(const AttentionArgs &a, uint32_t key0) const { return every(a, key0, kTileKeys); }
+    // does any row see one of the keys [key, key + count), do all rows see all of them?
+    __device__ inline bool any(const AttentionArgs &a, uint32_t key, uint32_t count) const {
+        return (int64_t)key <= most && (a.window == 0 || key < a.sinks || (int64_t)key + count - 1 > least - (int64_t)a.window);
+    }
+    __device__ inline bool every(const AttentionArgs &a, uint32_t key, uint32_t count) const {
+        return (int64_t)key + count - 1 <= least &&
+               (a.window == 0 || (int64_t)key > most - (int64_t)a.window || (uint64_t)key + count <= a.sinks);
     }
 };
 
@@ -191,7 +196,9 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
         uint32_t item = 0, slot = 0, lap = 0;
         uint32_t token = n > 0 ? token_of(0) : 0, page = n > 0 ? page_of(token) : 0;
         for (uint32_t j = 0; j < n && ok; ++j) {
-            const uint32_t held = min(kTileKeys, keys_end - u.key(j));
+            // the boxes that hold something which some row sees, a bit each: on the edges of a window most do not
+            const uint32_t wanted = __ballot_sync(0xffffffffu, (lane << shift) < kTileKeys && u.key(j) + my_token < keys_end &&
+                                                                   u.any(a, u.key(j) + my_token, 1u << shift));
             if (page >= a.cache.pages) {  // never followed: the pool's first page stands in for it
                 report(a.status, kBadPage);
                 page = 0;
@@ -207,15 +214,16 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     ok = false;
                     break;
                 }
-                const uint32_t first = keys ? 0 : part * S::v_rows;
-                const uint32_t boxes = first >= held ? 0 : (min(rows, held - first) + (1u << shift) - 1) >> shift;
+                const uint32_t first = keys ? 0 : part * S::v_rows >> shift, boxes = rows >> shift;
+                const uint32_t here = wanted >> first & ((1u << boxes) - 1);
                 const uint32_t bar = full0 + 8 * slot;
                 uint32_t to = to0 + slot * kSlotBytes;
-                if (leader) tc_mbar_expect_tx(bar, boxes * box_bytes);
+                if (leader) tc_mbar_expect_tx(bar, __popc(here) * box_bytes);
                 __syncwarp();
-                for (uint32_t box = 0; box < boxes; ++box, to += box_bytes)
-                    tc_tensor_copy_3d_by(leader, to, map, 0, __shfl_sync(0xffffffffu, line, (first >> shift) + box),
-                                         keys ? (int)part : 0, bar);
+                for (uint32_t box = 0; box < boxes; ++box, to += box_bytes) {
+                    const int y = __shfl_sync(0xffffffffu, line, first + box);
+                    if (here >> box & 1u) tc_tensor_copy_3d_by(leader, to, map, 0, y, keys ? (int)part : 0, bar);
+                }
                 ++item;
                 if (++slot == S::slots) {
                     slot = 0;
@@ -246,7 +254,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             const bool leader = tc_leader();
             const uint32_t to_s = __shfl_sync(0xffffffffu, tmem_s, 0), to_o = __shfl_sync(0xffffffffu, tmem_o, 0);
             const uint32_t rows0 = tc_smem_u32(query);
-            uint32_t k_slot = 0, k_lap = 0, v_slot = 0, v_lap = 0, looked = 0;
+            uint32_t k_slot = 0, k_lap = 0, v_slot = 0, v_lap = 0, looked = 0, begun = 0;
             auto advance = [](uint32_t &slot, uint32_t &lap) {
                 if (++slot == S::slots) {
                     slot = 0;
@@ -301,9 +309,12 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     const uint32_t values = v_ring + v_slot * kSlotBytes;
 #pragma unroll
                     for (uint32_t k = 0; k < S::v_rows / 16; ++k) {
+                        // keys that no row sees are left out, with whatever their place in the slot holds
+                        if (edge && !u.any(a, u.key(j) + part * S::v_rows + k * 16, 16)) continue;
                         tc_mma_by(leader, to_o, to_s + (j & 1) * 128 + (part * (S::v_rows / 16) + k) * 8,
                                   v_desc | at(values + ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 128),
-                                  o_idesc, j > 0 || part > 0 || k > 0 ? 1u : 0u);
+                                  o_idesc, begun);
+                        begun = 1;
                     }
                     tc_commit_by(leader, v_empty0 + 8 * v_slot);
                     advance(v_slot, v_lap);
@@ -317,26 +328,39 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     } else {
         // ---- query rows into shared memory, swizzled; a negative scale turns their sign, scale 0 makes them zero ----
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, hold = a.scale == 0.0f ? 0u : 0xffffffffu;
-        for (uint32_t i = threadIdx.x - 96; i < kTileRowsQ * (D / 8); i += kPromptThreads - 96) {
-            const uint32_t row = i / (D / 8), piece = i % (D / 8);
-            uint4 value = make_uint4(0, 0, 0, 0);
-            if (row < u.count) {
-                const uint32_t flat = u.row0 + row;
-                value = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
-                                                         (size_t)(u.rows.begin + flat / a.group) * a.ldq +
-                                                         (size_t)(u.head * a.group + flat % a.group) * D + piece * 8);
-                value = make_uint4((value.x ^ flip) & hold, (value.y ^ flip) & hold, (value.z ^ flip) & hold, (value.w ^ flip) & hold);
+        constexpr uint32_t kLoaders = kPromptThreads - 96, kAtOnce = 8;  // pieces of 16 bytes on their way per thread
+        const uint32_t q_thread = threadIdx.x - 96;
+#pragma unroll 1
+        for (uint32_t i0 = q_thread; i0 < kTileRowsQ * (D / 8); i0 += kLoaders * kAtOnce) {
+            uint4 value[kAtOnce];
+#pragma unroll
+            for (uint32_t e = 0; e < kAtOnce; ++e) {
+                const uint32_t row = (i0 + e * kLoaders) / (D / 8), piece = (i0 + e * kLoaders) % (D / 8);
+                value[e] = make_uint4(0, 0, 0, 0);
+                if (row < u.count) {
+                    const uint32_t flat = u.row0 + row;
+                    value[e] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
+                                                                (size_t)(u.rows.begin + flat / a.group) * a.ldq +
+                                                                (size_t)(u.head * a.group + flat % a.group) * D + piece * 8);
+                }
             }
-            *reinterpret_cast<uint4 *>(query + (piece >> 3) * (kTileRowsQ * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16)) = value;
+#pragma unroll
+            for (uint32_t e = 0; e < kAtOnce; ++e) {
+                const uint32_t row = (i0 + e * kLoaders) / (D / 8), piece = (i0 + e * kLoaders) % (D / 8);
+                if (row < kTileRowsQ)
+                    *reinterpret_cast<uint4 *>(query + (piece >> 3) * (kTileRowsQ * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16)) =
+                        make_uint4((value[e].x ^ flip) & hold, (value[e].y ^ flip) & hold, (value[e].z ^ flip) & hold,
+                                   (value[e].w ^ flip) & hold);
+            }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         tc_mbar_arrive(q_full);
 
         if (warp == 3) {
-            // ---- the values of masked tiles: zeros where no row sees them, no infinity where only some rows do ----
+            // ---- the values of masked tiles, in the steps of 16 keys that some rows see and others do not: zeros where no
+            // row sees them, no infinity where only some do ----
             constexpr uint32_t exponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
             constexpr uint32_t both = exponent | exponent << 16, low = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
-            constexpr uint32_t part_shift = S::parts == 4 ? 2 : S::parts == 2 ? 1 : 0;
             const int64_t window = a.window, sinks = a.sinks;
             uint32_t looked = 0;
             for (uint32_t j = 0; j < n && ok; ++j) {
@@ -348,18 +372,24 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 for (uint32_t part = 0; part < S::parts && ok; ++part) {
                     const uint32_t item = j * S::parts + part, slot = item % S::slots;
                     if (!tc_wait(v_full0 + 8 * slot, (item / S::slots) & 1)) { ok = false; break; }  // it is: acquires
-                    uint4 *const cells = reinterpret_cast<uint4 *>(ring + (S::slots + slot) * kSlotBytes);
-#pragma unroll 4
-                    for (uint32_t i = lane; i < kSlotBytes / 16; i += 32) {
+                    for (uint32_t k = 0; k < S::v_rows / 16; ++k) {
+                        const uint32_t key16 = key0 + part * S::v_rows + k * 16;
+                        if (!u.any(a, key16, 16) || u.every(a, key16, 16)) continue;
                         // [box][chunk][token of the box][8 cells]
-                        const uint32_t token = (i >> (p.v_shift + 3 + part_shift) << p.v_shift) + ((i >> 3) & ((1u << p.v_shift) - 1));
-                        const int64_t key = (int64_t)key0 + part * S::v_rows + token;
-                        if (key > u.most || (window != 0 && key <= u.least - window && key >= sinks)) {
-                            cells[i] = make_uint4(0, 0, 0, 0);
-                        } else if (!(key <= u.least && (window == 0 || key > u.most - window || key < sinks))) {
-                            // an exponent of all ones carries into the bit above it
-                            const uint4 c = cells[i];
-                            strange |= (((c.x & both) + low) | ((c.y & both) + low) | ((c.z & both) + low) | ((c.w & both) + low)) & 0x80008000u;
+                        uint4 *const cells = reinterpret_cast<uint4 *>(ring + (S::slots + slot) * kSlotBytes) +
+                                             ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 8;
+#pragma unroll 4
+                        for (uint32_t i = lane; i < 16 * 8 * S::parts; i += 32) {
+                            const uint32_t token = (i >> 3) & 15u, chunk = i >> 7;
+                            uint4 &cell = cells[(chunk << p.v_shift) * 8 + token * 8 + (i & 7)];
+                            const int64_t key = (int64_t)key16 + token;
+                            if (key > u.most || (window != 0 && key <= u.least - window && key >= sinks)) {
+                                cell = make_uint4(0, 0, 0, 0);
+                            } else if (!(key <= u.least && (window == 0 || key > u.most - window || key < sinks))) {
+                                // an exponent of all ones carries into the bit above it
+                                const uint4 c = cell;
+                                strange |= (((c.x & both) + low) | ((c.y & both) + low) | ((c.z & both) + low) | ((c.w & both) + low)) & 0x80008000u;
+                            }
                         }
                     }
                 }
