@@ -285,7 +285,9 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 // a masked tile's values are handed to the warp that looks at them and handed back: a strict exchange,
                 // so neither side can miss a round of a barrier that the other is already past
                 const bool edge = !u.clear(a, u.key(j));
+                uint32_t steps = 0xffu;  // of 16 keys that some row sees
                 if (edge) {
+                    steps = __ballot_sync(0xffffffffu, lane < kTileKeys / 16 && u.any(a, u.key(j) + lane * 16, 16));
                     uint32_t slot = v_slot, lap = v_lap;
 #pragma unroll
                     for (uint32_t part = 0; part < S::parts; ++part) {
@@ -310,7 +312,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
 #pragma unroll
                     for (uint32_t k = 0; k < S::v_rows / 16; ++k) {
                         // keys that no row sees are left out, with whatever their place in the slot holds
-                        if (edge && !u.any(a, u.key(j) + part * S::v_rows + k * 16, 16)) continue;
+                        if (!(steps >> (part * (S::v_rows / 16) + k) & 1u)) continue;
                         tc_mma_by(leader, to_o, to_s + (j & 1) * 128 + (part * (S::v_rows / 16) + k) * 8,
                                   v_desc | at(values + ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 128),
                                   o_idesc, begun);
@@ -361,35 +363,42 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             // row sees them, no infinity where only some do ----
             constexpr uint32_t exponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
             constexpr uint32_t both = exponent | exponent << 16, low = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
-            const int64_t window = a.window, sinks = a.sinks;
             uint32_t looked = 0;
             for (uint32_t j = 0; j < n && ok; ++j) {
                 const uint32_t key0 = u.key(j);
                 if (u.clear(a, key0)) continue;
-                if (!tc_wait(v_look, looked & 1)) { ok = false; break; }
+                // a bit per key: nobody sees it, some do and some do not; four words of 32 keys
+                uint32_t nobody[4], some[4];
+#pragma unroll
+                for (uint32_t w = 0; w < 4; ++w) {
+                    const bool any = u.any(a, key0 + 32 * w + lane, 1), every = u.every(a, key0 + 32 * w + lane, 1);
+                    nobody[w] = __ballot_sync(0xffffffffu, !any);
+                    some[w] = __ballot_sync(0xffffffffu, any && !every);
+                }
+                ok = tc_warp_wait(v_look, looked & 1);
+                if (!ok) break;
                 ++looked;
                 uint32_t strange = 0;
-                for (uint32_t part = 0; part < S::parts && ok; ++part) {
+#pragma unroll
+                for (uint32_t g = 0; g < kTileKeys / 16; ++g) {
+                    const uint32_t part = g * 16 / S::v_rows, k = g - part * (S::v_rows / 16);
                     const uint32_t item = j * S::parts + part, slot = item % S::slots;
-                    if (!tc_wait(v_full0 + 8 * slot, (item / S::slots) & 1)) { ok = false; break; }  // it is: acquires
-                    for (uint32_t k = 0; k < S::v_rows / 16; ++k) {
-                        const uint32_t key16 = key0 + part * S::v_rows + k * 16;
-                        if (!u.any(a, key16, 16) || u.every(a, key16, 16)) continue;
-                        // [box][chunk][token of the box][8 cells]
-                        uint4 *const cells = reinterpret_cast<uint4 *>(ring + (S::slots + slot) * kSlotBytes) +
-                                             ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 8;
-#pragma unroll 4
-                        for (uint32_t i = lane; i < 16 * 8 * S::parts; i += 32) {
-                            const uint32_t token = (i >> 3) & 15u, chunk = i >> 7;
-                            uint4 &cell = cells[(chunk << p.v_shift) * 8 + token * 8 + (i & 7)];
-                            const int64_t key = (int64_t)key16 + token;
-                            if (key > u.most || (window != 0 && key <= u.least - window && key >= sinks)) {
-                                cell = make_uint4(0, 0, 0, 0);
-                            } else if (!(key <= u.least && (window == 0 || key > u.most - window || key < sinks))) {
-                                // an exponent of all ones carries into the bit above it
-                                const uint4 c = cell;
-                                strange |= (((c.x & both) + low) | ((c.y & both) + low) | ((c.z & both) + low) | ((c.w & both) + low)) & 0x80008000u;
-                            }
+                    const uint32_t none = nobody[g >> 1] >> (g & 1) * 16 & 0xffffu, mixed = some[g >> 1] >> (g & 1) * 16 & 0xffffu;
+                    if (none == 0xffffu || (none | mixed) == 0) continue;  // not multiplied, or seen by all
+                    ok = ok && tc_warp_wait(v_full0 + 8 * slot, (item / S::slots) & 1);  // it is: acquires
+                    // [box][chunk][token of the box][8 cells]
+                    uint4 *const cells = reinterpret_cast<uint4 *>(ring + (S::slots + slot) * kSlotBytes) +
+                                         ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 8 + lane;
+#pragma unroll
+                    for (uint32_t i = 0; i < 4 * S::parts; ++i) {  // four tokens of a chunk at a time
+                        const uint32_t token = (i & 3) * 4 + (lane >> 3);
+                        uint4 &cell = cells[(i >> 2 << p.v_shift) * 8 + (i & 3) * 32];
+                        if (none >> token & 1u) {
+                            cell = make_uint4(0, 0, 0, 0);
+                        } else if (mixed >> token & 1u) {
+                            // an exponent of all ones carries into the bit above it
+                            const uint4 c = cell;
+                            strange |= (((c.x & both) + low) | ((c.y & both) + low) | ((c.z & both) + low) | ((c.w & both) + low)) & 0x80008000u;
                         }
                     }
                 }
@@ -485,10 +494,11 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 total = exchange[row] + exchange[128 + row];
             }
             // ---- output, or sums for the cluster ----
-            const uint32_t flat = u.row0 + row;
             if (p.splits == 1) {
+                // through shared memory (the ring is done with): a row leaves in whole lines, not 64 bytes at a time per thread
                 const float over = total == 0.0f ? 0.0f : 1.0f / total;
                 if (active) {
+                    uint4 *const staged = reinterpret_cast<uint4 *>(ring);  // [128][D / 8], pieces turned by the row
 #pragma unroll 1
                     for (uint32_t column = half * (D / 2); column < (half + 1) * (D / 2); column += 32) {
                         uint32_t o[32];
@@ -499,18 +509,28 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] = 0;
                         }
-                        if (row < u.count) {
-                            T *to = static_cast<T *>(a.out) + (size_t)(u.rows.begin + flat / a.group) * a.ldo +
-                                    (size_t)(u.head * a.group + flat % a.group) * D + column;
 #pragma unroll
-                            for (int i = 0; i < 32; i += 8) {
-                                uint4 packed;
-                                uint32_t *const w = reinterpret_cast<uint32_t *>(&packed);
+                        for (int i = 0; i < 32; i += 8) {
+                            uint4 packed;
+                            uint32_t *const w = reinterpret_cast<uint32_t *>(&packed);
 #pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    w[k] = pack2<T>(__uint_as_float(o[i + 2 * k]) * over, __uint_as_float(o[i + 2 * k + 1]) * over);
-                                *reinterpret_cast<uint4 *>(to + i) = packed;
-                            }
+                            for (int k = 0; k < 4; ++k)
+                                w[k] = pack2<T>(__uint_as_float(o[i + 2 * k]) * over, __uint_as_float(o[i + 2 * k + 1]) * over);
+                            staged[row * (D / 8) + (((column + i) >> 3) ^ (row & 7))] = packed;
+                        }
+                    }
+                    pair_barrier(1 + quad);
+                    // the pair's 32 rows, 64 lanes over their pieces
+                    constexpr uint32_t kRowsAtOnce = 64 / (D / 8);
+                    const uint32_t lane64 = half * 32 + lane, piece = lane64 % (D / 8);
+#pragma unroll 4
+                    for (uint32_t r = lane64 / (D / 8); r < 32; r += kRowsAtOnce) {
+                        const uint32_t out_row = quad * 32 + r;
+                        if (out_row < u.count) {
+                            const uint32_t out_flat = u.row0 + out_row;
+                            T *const to = static_cast<T *>(a.out) + (size_t)(u.rows.begin + out_flat / a.group) * a.ldo +
+                                          (size_t)(u.head * a.group + out_flat % a.group) * D + piece * 8;
+                            *reinterpret_cast<uint4 *>(to) = staged[out_row * (D / 8) + (piece ^ (out_row & 7))];
                         }
                     }
                 }
