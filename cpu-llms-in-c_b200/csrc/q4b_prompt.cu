@@ -693,30 +693,44 @@ cudaError_t launch_prompt_of(const AttentionArgs &args, int sm_count, cudaStream
     const uint64_t tiles = (uint64_t)args.batch.tokens * args.group / kTileRowsQ +
                            (args.batch.sequences < args.batch.tokens ? args.batch.sequences : args.batch.tokens);
     const uint64_t units = tiles * args.cache.kv_heads;
-    p.splits = 1;
-    while (p.splits < kMostSplits && units * (p.splits + 1) <= (uint64_t)sm_count) ++p.splits;
-    if (units * p.splits > 0x7fffffffu) return cudaErrorInvalidConfiguration;
-    p.units = (uint32_t)units;
     const size_t smem = S::query + (size_t)2 * S::slots * kSlotBytes + kMiscBytes + 1024;
-    static bool configured[kMaxDevices] = {};
-    const int slot = device_slot();
-    if (slot < 0 || !configured[slot]) {
-        cudaError_t status = cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (status != cudaSuccess) return status;
-        if (slot >= 0) configured[slot] = true;
-    }
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3((unsigned)(units * p.splits));
     config.blockDim = dim3(kPromptThreads);
     config.dynamicSmemBytes = smem;
     config.stream = stream;
     cudaLaunchAttribute attribute[1];
     attribute[0].id = cudaLaunchAttributeClusterDimension;
-    attribute[0].val.clusterDim.x = p.splits;
+    attribute[0].val.clusterDim.x = 1;
     attribute[0].val.clusterDim.y = 1;
     attribute[0].val.clusterDim.z = 1;
     config.attrs = attribute;
     config.numAttrs = 1;
+    // clusters of 2 .. 8 that a device holds at once: fewer than its SMs divided, a cluster stays within a part of the chip
+    static int room[kMaxDevices][kMostSplits + 1] = {};
+    int here[kMostSplits + 1] = {};
+    const int slot = device_slot();
+    if (slot >= 0 && room[slot][1] != 0) {
+        for (uint32_t k = 1; k <= kMostSplits; ++k) here[k] = room[slot][k];
+    } else {
+        cudaError_t status = cudaFuncSetAttribute(prompt_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (status != cudaSuccess) return status;
+        here[1] = sm_count;
+        for (uint32_t k = 2; k <= kMostSplits; ++k) {
+            attribute[0].val.clusterDim.x = k;
+            config.gridDim = dim3((unsigned)sm_count / k * k);
+            status = cudaOccupancyMaxActiveClusters(&here[k], prompt_kernel<T, D>, &config);
+            if (status != cudaSuccess) return status;
+        }
+        if (slot >= 0)
+            for (uint32_t k = kMostSplits; k >= 1; --k) room[slot][k] = here[k];
+    }
+    p.splits = 1;
+    for (uint32_t k = 2; k <= kMostSplits; ++k)
+        if (units <= (uint64_t)here[k]) p.splits = k;
+    if (units * p.splits > 0x7fffffffu) return cudaErrorInvalidConfiguration;
+    p.units = (uint32_t)units;
+    config.gridDim = dim3((unsigned)(units * p.splits));
+    attribute[0].val.clusterDim.x = p.splits;
     return cudaLaunchKernelEx(&config, prompt_kernel<T, D>, p);
 }
 
