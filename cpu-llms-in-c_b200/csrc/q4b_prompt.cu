@@ -416,6 +416,9 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             const int64_t place = row < u.count ? u.place0 + (u.row0 + row) / a.group : -1;
             float top = -INFINITY, total = 0.0f;
             for (uint32_t j = 0; j < n; ++j) {
+                // found out while S(j) is on its way: are there columns to hide, and which
+                const uint32_t key0 = u.key(j);
+                const bool edge = !u.clear(a, key0);
                 if (ok && !tc_wait(s_full0 + 8 * (j & 1), (j >> 1) & 1)) ok = false;
                 tc_fence_after();
                 const uint32_t s_columns = tmem_s + (j & 1) * 128 + lanes;
@@ -423,22 +426,23 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     uint32_t raw[2][32];
                     tc_load_32(s_columns + half * 64, raw[0]);
                     tc_load_32(s_columns + half * 64 + 32, raw[1]);
-                    tc_wait_load();
-                    const uint32_t key0 = u.key(j);
-                    if (!u.clear(a, key0)) {
-                        // visible columns: below `high`, and from `low` on or below `sink`
+                    tc_wait_loaded(raw[0]);
+                    tc_wait_loaded(raw[1]);
+                    if (edge) {
+                        // visible columns: below `behind`, and from `from` on or below `sink`
                         const int64_t first = (int64_t)key0 + half * 64;
-                        const int32_t high = (int32_t)max((int64_t)0, min((int64_t)64, place + 1 - first));
-                        const int32_t low = a.window == 0 ? 0 : (int32_t)max((int64_t)0, min((int64_t)64, place - (int64_t)a.window + 1 - first));
+                        const int32_t behind = (int32_t)max((int64_t)0, min((int64_t)64, place + 1 - first));
+                        const int32_t from = a.window == 0 ? 0 : (int32_t)max((int64_t)0, min((int64_t)64, place - (int64_t)a.window + 1 - first));
                         const int32_t sink = (int32_t)max((int64_t)0, min((int64_t)64, (int64_t)a.sinks - first));
 #pragma unroll
                         for (int i = 0; i < 64; ++i) {
-                            if (!(i < high && (i >= low || i < sink))) raw[i >> 5][i & 31] = 0xff800000u;  // -infinity
+                            if (!(i < behind && (i >= from || i < sink))) raw[i >> 5][i & 31] = 0xff800000u;  // -infinity
                         }
                     }
-                    float high = -INFINITY;
+                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) high = fmaxf(high, __uint_as_float(raw[i >> 5][i & 31]));
+                    for (int i = 0; i < 64; ++i) most[i & 3] = fmaxf(most[i & 3], __uint_as_float(raw[i >> 5][i & 31]));
+                    float high = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
                     pair_barrier(5 + quad);  // the other half has read what it was told last time
                     exchange[half * 128 + row] = high;
                     pair_barrier(1 + quad);
@@ -457,7 +461,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                             for (uint32_t column = half * (D / 2); column < (half + 1) * (D / 2); column += 32) {
                                 uint32_t o[32];
                                 tc_load_32(tmem_o + lanes + column, o);
-                                tc_wait_load();
+                                tc_wait_loaded(o);
 #pragma unroll
                                 for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
                                 tc_store_32(tmem_o + lanes + column, o);
@@ -466,13 +470,15 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     }
                     const float minus = top == -INFINITY ? 0.0f : -top;
                     uint32_t weights[32];
+                    float sum[2] = {0.0f, 0.0f};
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
                         const float x = exp2_of(fmaf(__uint_as_float(raw[i >> 4][(2 * i) & 31]), c, minus));
                         const float y = exp2_of(fmaf(__uint_as_float(raw[i >> 4][(2 * i + 1) & 31]), c, minus));
-                        total += x + y;
+                        sum[i & 1] += x + y;
                         weights[i] = pack2<T>(x, y);
                     }
+                    total += sum[0] + sum[1];
                     tc_store_32(s_columns + half * 32, weights);
                     tc_wait_store();
                     // O(j - 1) is complete long before P(j) is needed; every warp sees every round of its barrier
@@ -504,7 +510,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                         uint32_t o[32];
                         if (n > 0) {
                             tc_load_32(tmem_o + lanes + column, o);
-                            tc_wait_load();
+                            tc_wait_loaded(o);
                         } else {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) o[i] = 0;
@@ -541,7 +547,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     uint32_t o[32];
                     if (n > 0) {
                         tc_load_32(tmem_o + lanes + column, o);
-                        tc_wait_load();
+                        tc_wait_loaded(o);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = 0;
