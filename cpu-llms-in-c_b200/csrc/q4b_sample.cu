@@ -59,6 +59,7 @@ struct SampleShared {
         uint64_t list[kListed];            // composites
         uint64_t mass[kBins];
     };
+    uint2 queue[16][64];                   // per warp: values and indices that wait for 31 others
     uint64_t sums[kListed];                // their weights; before that, what this block puts on the list
 };
 
@@ -179,6 +180,51 @@ struct Slice {
             }
         }
     }
+    // f over the values of a tile that may be `bound` or more (a NaN may), as a warp: they are collected and f runs for 32 at
+    // a time, so a pass over a row of which little matters costs a comparison per value and f for those that do
+    template <typename F> __device__ inline void tile_above(uint32_t t, float bound, uint2 *queue, F f) const {
+        const uint4 *const from = reinterpret_cast<const uint4 *>(data + head);
+        const uint32_t lane = threadIdx.x & 31, below = (1u << lane) - 1;
+        uint32_t w = t * kTileWords + lane, waiting = 0;
+        uint4 next = w < words ? from[w] : make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+        for (uint32_t r = 0; r < kTileRows4; ++r, w += 32) {
+            const uint4 word = next;
+            const bool here = w < words;
+            if (r + 1 < kTileRows4 && w + 32 < words) next = from[w + 32];
+            const T *x = reinterpret_cast<const T *>(&word);
+#pragma unroll
+            for (uint32_t j = 0; j < kWord; ++j) {
+                const float value = as_float(x[j]);
+                const bool takes = here && !(value < bound);
+                const uint32_t mask = __ballot_sync(0xffffffffu, takes);
+                if (mask == 0) continue;
+                if (takes) queue[waiting + __popc(mask & below)] = make_uint2(__float_as_uint(value), head + w * kWord + j);
+                waiting += __popc(mask);
+                if (waiting >= 32) {
+                    __syncwarp();
+                    const uint2 own = queue[lane], rest = queue[32 + lane];
+                    __syncwarp();
+                    waiting -= 32;
+                    if (lane < waiting) queue[lane] = rest;
+                    f(__uint_as_float(own.x), own.y);
+                }
+            }
+        }
+        __syncwarp();
+        if (lane < waiting) f(__uint_as_float(queue[lane].x), queue[lane].y);
+        __syncwarp();
+    }
+    // the same over the whole slice, as a block
+    template <typename F> __device__ inline void each_above(float bound, uint2 *queue, F f) const {
+        const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll 1
+        for (uint32_t t = warp; t < tiles(); t += (blockDim.x / 32)) tile_above(t, bound, queue, f);
+        if (warp == 0 && lane < head + tail) {
+            const uint32_t i = lane < head ? lane : size - tail + (lane - head);
+            if (!(at(i) < bound)) f(at(i), i);
+        }
+    }
     // f over the whole slice, as a block
     template <typename F> __device__ inline void each(F f) const {
         const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -191,15 +237,28 @@ struct Slice {
     }
 };
 
-// Weights by the distance to the largest logit: about 45 instructions, which are what a pass costs.
+// Weights by the distance to the largest logit: about 45 instructions, which are what a pass costs, in one chain from the
+// logit to the weight.  Without a branch in it several values' chains run side by side; with two the pass took 70 clocks
+// per 32 values and scheduler, each chain waiting for the one before.
 struct Weigh {
     const uint2 *power;
-    float high, rate, rate_low;  // log2(e) / temperature = rate + rate_low, finite
+    float high, rate, rate_low;  // log2(e) / temperature = rate + rate_low; all finite
+    bool narrow;                 // 16-bit logits: fp32 holds their differences (but of tiny ones to huge ones)
+    __device__ inline void set(float largest, float temperature) {
+        const double exact = 1.4426950408889634074 / (double)temperature;
+        high = largest;
+        rate = fminf((float)exact, 3.0e38f);
+        rate_low = rate < 3.0e38f ? (float)(exact - (double)rate) : 0.0f;
+        if (largest == INFINITY) {  // its equals share everything: they become the largest number, everything else is far away
+            high = 3.402823466e38f;
+            rate = 1.0f;
+            rate_low = 0.0f;
+        }
+    }
     // of distance + distance_low >= 0; beyond 2^-43, overflow and NaN are nothing
     __device__ inline uint64_t at(float distance, float distance_low) const {
         const float y = distance * rate;
-        if (!(y < 43.0f)) return 0;
-        const float y_low = fmaf(distance, rate, -y) + fmaf(distance, rate_low, distance_low * rate);
+        const float y_low = fmaf(distance, rate_low, fmaf(distance, rate, -y)) + distance_low * rate;
         const float shifted = fmaf(y, 256.0f, 12582912.0f);  // 1.5 x 2^23: the nearest whole number of 1/256
         const uint32_t k = __float_as_uint(shifted) - 0x4b400000u;
         const float rest = fmaf(shifted - 12582912.0f, -1.0f / 256.0f, y) + y_low;
@@ -207,14 +266,17 @@ struct Weigh {
         const float more = q * fmaf(q, fmaf(q, 0.16666667f, 0.5f), 1.0f);  // 2^-rest - 1; q^4 / 24 < 2^-42
         const uint2 base = power[k & 255u];
         const uint32_t value = base.x + __float_as_uint(fmaf(__uint_as_float(base.y), more, 12582912.0f)) - 0x4b400000u;
-        const uint32_t n = k >> 8;
-        return (((uint64_t)value << 11) + ((1ull << n) >> 1)) >> n;
+        const uint32_t n = k >> 8 & 63u;
+        const uint64_t weight = (((uint64_t)value << 11) + ((1ull << n) >> 1)) >> n;
+        return y < 43.0f ? weight : 0;
     }
     __device__ inline uint64_t of(float x) const {
-        if (x == high) return kOne;
-        const float d = high - x;
+        float own;  // at most the largest (an infinity), a NaN stays one
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(own) : "f"(x), "f"(high));
+        const float d = high - own;
+        if (narrow) return at(d, 0.0f);
         const float back = high - d;          // d + low = high - x exactly
-        const float low = (high - (d + back)) + (back - x);
+        const float low = (high - (d + back)) + (back - own);
         return at(d, low);
     }
 };
@@ -268,17 +330,20 @@ __device__ inline uint64_t reach_of(float share, uint64_t total) {
 }
 
 // The elements that `wanted` names, as composites in the list of the cluster's first block; how many there are, or
-// 0xffffffff when they are too many for it; `bound` is less than any of them, or -infinity.  A block lists its own first: a place in another block's list is a round trip.
-template <typename T, typename F>
+// 0xffffffff when they are too many for it; `bound` is less than any of them, or -infinity (COLLECT: `wanted` is long
+// and some per cent of the row pass the bound).  A block lists its own first: a place in another block's list is a round trip.
+template <bool COLLECT, typename T, typename F>
 __device__ uint32_t gather(cg::cluster_group &cluster, SampleShared &sh, const Slice<T> &slice, float bound, F wanted) {
     if (threadIdx.x == 0) sh.own_listed = 0;
     __syncthreads();
-    slice.each([&](float x, uint32_t i) {
-        if (!(x < bound) && wanted(x, i)) {  // one comparison for most
+    auto list = [&](float x, uint32_t i) {
+        if (wanted(x, i)) {
             const uint32_t place = atomicAdd(&sh.own_listed, 1u);
             if (place < kListed) sh.sums[place] = composite(x, slice.begin + i);
         }
-    });
+    };
+    if (COLLECT) slice.each_above(bound, sh.queue[threadIdx.x >> 5], list);
+    else slice.each([&](float x, uint32_t i) { if (!(x < bound)) list(x, i); });
     __syncthreads();
     const uint32_t own = sh.own_listed, blocks = cluster.num_blocks(), rank = cluster.block_rank();
     if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->span_high[rank] = own;
@@ -304,14 +369,14 @@ __device__ uint32_t gather(cg::cluster_group &cluster, SampleShared &sh, const S
 // of those at or above `floor`.  By mass: the first at which the running weight reaches `wanted`.
 template <bool MASS, typename T>
 __device__ __noinline__ uint64_t find_cut(cg::cluster_group &cluster, SampleShared &sh, const Slice<T> &slice, const Weigh &weigh,
-                             float to_bin, uint32_t bins, uint64_t floor, uint64_t wanted) {
+                             float high, float to_bin, uint32_t bins, uint64_t floor, uint64_t wanted) {
     const uint32_t blocks = cluster.num_blocks(), rank = cluster.block_rank();
     bool by_distance = true;
     uint64_t span_low = floor, span_high = ~0ull;  // composites still in question, and how they are cut into bins
     uint32_t shift = 0;
     uint64_t before = 0;                           // count or mass above the span
     auto bin_of = [&](float x, uint64_t c) -> uint32_t {
-        return by_distance ? whole(place_of(x, weigh.high, to_bin, (float)(bins - 1))) : (uint32_t)((span_high - c) >> shift);
+        return by_distance ? whole(place_of(x, high, to_bin, (float)(bins - 1))) : (uint32_t)((span_high - c) >> shift);
     };
     auto in_span = [&](uint64_t c) { return c >= span_low && c <= span_high; };
     for (;;) {
@@ -350,7 +415,7 @@ __device__ __noinline__ uint64_t find_cut(cg::cluster_group &cluster, SampleShar
         before = sh.found_before;
         if (border_count <= kListed) {
             // gather the bin in the first block and rank it there
-            gather(cluster, sh, slice, -INFINITY, [&](float x, uint32_t i) {
+            gather<false>(cluster, sh, slice, -INFINITY, [&](float x, uint32_t i) {
                 const uint64_t c = composite(x, slice.begin + i);
                 return in_span(c) && bin_of(x, c) == border;
             });
@@ -659,10 +724,8 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     }
     Weigh weigh;
     weigh.power = sh.power;
-    weigh.high = high;
-    const double rate = 1.4426950408889634074 / (double)temperature;
-    weigh.rate = fminf((float)rate, 3.0e38f);
-    weigh.rate_low = weigh.rate < 3.0e38f ? (float)(rate - (double)weigh.rate) : 0.0f;
+    weigh.narrow = sizeof(T) == 2;
+    weigh.set(high, temperature);
     const uint32_t bins = min(kBins, blocks * blockDim.x);
     const float last_bin = (float)(bins - 1), to_bin = last_bin / fmaxf(high - low, 1e-30f);
     const uint32_t k = asked_k < p.vocab ? asked_k : 0;
@@ -698,8 +761,8 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         cluster.sync();
         if (sh.found_count != 0) {  // fewer threads than k otherwise
             const float end = (float)(sh.high_bin + 1);
-            if (gather(cluster, sh, slice, value_below(end), [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; }) <=
-                kListed) {
+            if (gather<false>(cluster, sh, slice, value_below(end),
+                              [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; }) <= kListed) {
                 if (rank == 0) finish_list(p, row, sh, weigh, k, share, 0, least, uniform);
                 return;
             }
@@ -711,13 +774,16 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         // ---- counts ----
         const bool add = k == 0;  // top-p alone is a share of everything
         uint64_t mine = 0;
-        slice.each([&](float x, uint32_t) {
-            atomicAdd(&sh.count[whole(place_of(x, high, to_bin, last_bin))], 1u);
-            if (add) mine += weigh.of(x);
-        });
+        auto count = [&](float x) { atomicAdd(&sh.count[whole(place_of(x, high, to_bin, last_bin))], 1u); };
         if (add) {
+            slice.each([&](float x, uint32_t) {
+                count(x);
+                mine += weigh.of(x);
+            });
             mine = block_sum(mine, sh.warp_values);
             if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->total[rank] = mine;
+        } else {
+            slice.each([&](float x, uint32_t) { count(x); });
         }
         if (threadIdx.x == 0) {
             sh.low_bin = sh.high_bin = bins - 1;
@@ -775,7 +841,8 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         if (down_to != 0 && down_to <= kListed) {
             // ---- few stay ----
             const float end = (float)(high_bin + 1);
-            gather(cluster, sh, slice, value_below(end), [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; });
+            gather<false>(cluster, sh, slice, value_below(end),
+                          [&](float x, uint32_t) { return place_of(x, high, to_bin, last_bin) < end; });
             if (rank == 0) finish_list(p, row, sh, weigh, k, share, everything, least, uniform);
             return;
         }
@@ -815,7 +882,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             // ---- many stay, few lie in the bracket: those are put in order ----
             const float first = (float)low_bin, end = (float)(high_bin + 1);
             uint64_t above = 0, all_above;
-            gather(cluster, sh, slice, value_below(end), [&](float x, uint32_t) {
+            gather<true>(cluster, sh, slice, value_below(end), [&](float x, uint32_t) {
                 const float v = place_of(x, high, to_bin, last_bin);
                 if (v < first) above += weigh.of(x);
                 return v >= first && v < end;
@@ -834,7 +901,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             const float first = (float)low_bin, end = (float)(high_bin + 1), finer = (float)bins / (end - first);
             uint64_t above = 0;
             auto fine_bin = [&](float v) { return whole(fminf((v - first) * finer, last_bin)); };
-            slice.each([&](float x, uint32_t) {
+            slice.each_above(value_below(end), sh.queue[warp], [&](float x, uint32_t) {
                 const float v = place_of(x, high, to_bin, last_bin);
                 if (v >= end) return;
                 const uint64_t w = weigh.of(x);
@@ -866,16 +933,16 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             const uint32_t border = sh.fine_bin, border_count = sh.fine_count;
             const uint64_t before = sh.found_before;
             if (border_count != 0 && border_count <= kListed) {
-                gather(cluster, sh, slice, value_below(end), [&](float x, uint32_t) {
+                gather<true>(cluster, sh, slice, value_below(end), [&](float x, uint32_t) {
                     const float v = place_of(x, high, to_bin, last_bin);
                     return v >= first && v < end && fine_bin(v) == border;
                 });
                 cut = rank_list(before);
             } else {
-                cut = find_cut<true>(cluster, sh, slice, weigh, to_bin, bins, 0ull, wanted);
+                cut = find_cut<true>(cluster, sh, slice, weigh, high, to_bin, bins, 0ull, wanted);
             }
         } else {
-            cut = find_cut<false>(cluster, sh, slice, weigh, to_bin, bins, 0ull, wanted);
+            cut = find_cut<false>(cluster, sh, slice, weigh, high, to_bin, bins, 0ull, wanted);
             if (share < 1.0f) {
                 mine = 0;
                 slice.each([&](float x, uint32_t i) {
@@ -885,13 +952,14 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
                 if (threadIdx.x < blocks) cluster.map_shared_rank(&sh, threadIdx.x)->total[rank] = mine;
                 cluster.sync();
                 for (uint32_t r = 0; r < blocks; ++r) everything += sh.total[r];
-                cut = find_cut<true>(cluster, sh, slice, weigh, to_bin, bins, cut, reach_of(share, everything));
+                cut = find_cut<true>(cluster, sh, slice, weigh, high, to_bin, bins, cut, reach_of(share, everything));
             }
         }
     }
 
     // ---- the token: sums per tile (the head is one of its own in front, the tail one behind) ----
     const bool all = cut == 0;
+    const float cut_logit = all ? -INFINITY : logit_of(cut);
     auto kept = [&](float x, uint32_t i) -> uint64_t {
         if (!all && composite(x, slice.begin + i) < cut) return 0;
         const uint64_t w = weigh.of(x);
@@ -905,7 +973,9 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         } else if (t == tile_count - 1) {
             if (lane < slice.tail) sum = kept(slice.at(slice.size - slice.tail + lane), slice.size - slice.tail + lane);
         } else {
-            slice.tile(t - 1, [&](float x, uint32_t i) { sum += kept(x, i); });
+            if (all && least == 0) slice.tile(t - 1, [&](float x, uint32_t) { sum += weigh.of(x); });
+            else if (all) slice.tile(t - 1, [&](float x, uint32_t i) { sum += kept(x, i); });
+            else slice.tile_above(t - 1, cut_logit, sh.queue[warp], [&](float x, uint32_t i) { sum += kept(x, i); });
         }
         sum = warp_sum(sum);
         if (lane == 0) tiles[t] = sum;
