@@ -389,16 +389,25 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     // [box][chunk][token of the box][8 cells]
                     uint4 *const cells = reinterpret_cast<uint4 *>(ring + (S::slots + slot) * kSlotBytes) +
                                          ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 8 + lane;
+                    // four tokens of a chunk at a time, all on their way at once
+                    uint4 cell[4 * S::parts];
 #pragma unroll
-                    for (uint32_t i = 0; i < 4 * S::parts; ++i) {  // four tokens of a chunk at a time
-                        const uint32_t token = (i & 3) * 4 + (lane >> 3);
-                        uint4 &cell = cells[(i >> 2 << p.v_shift) * 8 + (i & 3) * 32];
+                    for (uint32_t i = 0; i < 4 * S::parts; ++i) cell[i] = cells[(i >> 2 << p.v_shift) * 8 + (i & 3) * 32];
+                    uint32_t found[4] = {0, 0, 0, 0};
+#pragma unroll
+                    for (uint32_t i = 0; i < 4 * S::parts; ++i) {
+                        // an exponent of all ones carries into the bit above it
+                        const uint4 &c = cell[i];
+                        found[i & 3] |= ((c.x & both) + low) | ((c.y & both) + low) | ((c.z & both) + low) | ((c.w & both) + low);
+                    }
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) {
+                        const uint32_t token = i * 4 + (lane >> 3);
+                        strange |= mixed >> token & 1u ? found[i] & 0x80008000u : 0;
                         if (none >> token & 1u) {
-                            cell = make_uint4(0, 0, 0, 0);
-                        } else if (mixed >> token & 1u) {
-                            // an exponent of all ones carries into the bit above it
-                            const uint4 c = cell;
-                            strange |= (((c.x & both) + low) | ((c.y & both) + low) | ((c.z & both) + low) | ((c.w & both) + low)) & 0x80008000u;
+#pragma unroll
+                            for (uint32_t chunk = 0; chunk < S::parts; ++chunk)
+                                cells[(chunk << p.v_shift) * 8 + i * 32] = make_uint4(0, 0, 0, 0);
                         }
                     }
                 }
