@@ -74,6 +74,21 @@ __device__ inline float wide(__half x) { return __half2float(x); }
 __device__ inline float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
 __device__ inline void pair_barrier(uint32_t id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
+// (token, query head of the group) of every `step`th row, without a division for each
+struct RowWalk {
+    uint32_t token, member, group, step_tokens, step_members;
+    __device__ inline RowWalk(uint32_t flat, uint32_t of, uint32_t step)
+        : token(flat / of), member(flat % of), group(of), step_tokens(step / of), step_members(step % of) {}
+    __device__ inline void next() {
+        token += step_tokens;
+        member += step_members;
+        if (member >= group) {
+            member -= group;
+            ++token;
+        }
+    }
+};
+
 // What a thread block works on.
 struct Unit {
     SequenceRows rows;
@@ -331,26 +346,26 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
         // ---- query rows into shared memory, swizzled; a negative scale turns their sign, scale 0 makes them zero ----
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u, hold = a.scale == 0.0f ? 0u : 0xffffffffu;
         constexpr uint32_t kLoaders = kPromptThreads - 96, kAtOnce = 8;  // pieces of 16 bytes on their way per thread
-        const uint32_t q_thread = threadIdx.x - 96;
+        constexpr uint32_t kStep = kLoaders / (D / 8);                   // rows between a thread's pieces, all in one column
+        static_assert(kLoaders % (D / 8) == 0, "whole rows per round");
+        uint32_t row = (threadIdx.x - 96) / (D / 8);
+        const uint32_t piece = (threadIdx.x - 96) % (D / 8);
+        RowWalk at(u.row0 + row, a.group, kStep);
+        const T *const from = static_cast<const T *>(a.q) + (size_t)u.rows.begin * a.ldq + (size_t)u.head * a.group * D + piece * 8;
 #pragma unroll 1
-        for (uint32_t i0 = q_thread; i0 < kTileRowsQ * (D / 8); i0 += kLoaders * kAtOnce) {
+        for (; row < kTileRowsQ; row += kStep * kAtOnce) {
             uint4 value[kAtOnce];
 #pragma unroll
-            for (uint32_t e = 0; e < kAtOnce; ++e) {
-                const uint32_t row = (i0 + e * kLoaders) / (D / 8), piece = (i0 + e * kLoaders) % (D / 8);
+            for (uint32_t e = 0; e < kAtOnce; ++e, at.next()) {
                 value[e] = make_uint4(0, 0, 0, 0);
-                if (row < u.count) {
-                    const uint32_t flat = u.row0 + row;
-                    value[e] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.q) +
-                                                                (size_t)(u.rows.begin + flat / a.group) * a.ldq +
-                                                                (size_t)(u.head * a.group + flat % a.group) * D + piece * 8);
-                }
+                if (row + e * kStep < u.count)
+                    value[e] = *reinterpret_cast<const uint4 *>(from + (size_t)at.token * a.ldq + at.member * D);
             }
 #pragma unroll
             for (uint32_t e = 0; e < kAtOnce; ++e) {
-                const uint32_t row = (i0 + e * kLoaders) / (D / 8), piece = (i0 + e * kLoaders) % (D / 8);
-                if (row < kTileRowsQ)
-                    *reinterpret_cast<uint4 *>(query + (piece >> 3) * (kTileRowsQ * 128) + row * 128 + (((piece & 7) ^ (row & 7)) * 16)) =
+                const uint32_t r = row + e * kStep;
+                if (r < kTileRowsQ)
+                    *reinterpret_cast<uint4 *>(query + (piece >> 3) * (kTileRowsQ * 128) + r * 128 + (((piece & 7) ^ (r & 7)) * 16)) =
                         make_uint4((value[e].x ^ flip) & hold, (value[e].y ^ flip) & hold, (value[e].z ^ flip) & hold,
                                    (value[e].w ^ flip) & hold);
             }
@@ -537,16 +552,15 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     pair_barrier(1 + quad);
                     // the pair's 32 rows, 64 lanes over their pieces
                     constexpr uint32_t kRowsAtOnce = 64 / (D / 8);
-                    const uint32_t lane64 = half * 32 + lane, piece = lane64 % (D / 8);
+                    const uint32_t lane64 = half * 32 + lane, out_piece = lane64 % (D / 8), out_row0 = quad * 32 + lane64 / (D / 8);
+                    RowWalk out_at(u.row0 + out_row0, a.group, kRowsAtOnce);
+                    T *const to = static_cast<T *>(a.out) + (size_t)u.rows.begin * a.ldo + (size_t)u.head * a.group * D + out_piece * 8;
 #pragma unroll 4
-                    for (uint32_t r = lane64 / (D / 8); r < 32; r += kRowsAtOnce) {
-                        const uint32_t out_row = quad * 32 + r;
-                        if (out_row < u.count) {
-                            const uint32_t out_flat = u.row0 + out_row;
-                            T *const to = static_cast<T *>(a.out) + (size_t)(u.rows.begin + out_flat / a.group) * a.ldo +
-                                          (size_t)(u.head * a.group + out_flat % a.group) * D + piece * 8;
-                            *reinterpret_cast<uint4 *>(to) = staged[out_row * (D / 8) + (piece ^ (out_row & 7))];
-                        }
+                    for (uint32_t r = 0; r < 32 / kRowsAtOnce; ++r, out_at.next()) {
+                        const uint32_t out_row = out_row0 + r * kRowsAtOnce;
+                        if (out_row < u.count)
+                            *reinterpret_cast<uint4 *>(to + (size_t)out_at.token * a.ldo + out_at.member * D) =
+                                staged[out_row * (D / 8) + (out_piece ^ (out_row & 7))];
                     }
                 }
             } else if (active) {
