@@ -718,9 +718,14 @@ cudaError_t launch_prompt_of(const AttentionArgs &args, int sm_count, cudaStream
                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
             return cudaErrorInvalidValue;
     }
-    // as many tiles of rows as the host's numbers allow: full ones, and one ragged one per sequence
-    const uint64_t tiles = (uint64_t)args.batch.tokens * args.group / kTileRowsQ +
-                           (args.batch.sequences < args.batch.tokens ? args.batch.sequences : args.batch.tokens);
+    // As many tiles of rows as the host's numbers allow.  A sequence of n tokens has 1 + floor((n G - 1) / 128): the sum over
+    // s sequences of N tokens is at most s + floor((N G - s) / 128), and, as a further tile takes floor(128 / G) further
+    // tokens, at most s + floor((N - s) / floor(128 / G)).
+    const uint64_t tokens = args.batch.tokens, group = args.group;
+    const uint64_t sequences = args.batch.sequences < tokens ? args.batch.sequences : tokens;
+    uint64_t tiles = sequences + (tokens * group - sequences) / kTileRowsQ;
+    if (group <= kTileRowsQ && (tokens - sequences) / (kTileRowsQ / group) < (tokens * group - sequences) / kTileRowsQ)
+        tiles = sequences + (tokens - sequences) / (kTileRowsQ / group);
     const uint64_t units = tiles * args.cache.kv_heads;
     const size_t smem = S::query + (size_t)2 * S::slots * kSlotBytes + kMiscBytes + 1024;
     cudaLaunchConfig_t config = {};

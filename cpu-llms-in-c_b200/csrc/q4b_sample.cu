@@ -740,6 +740,8 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
     };
 
     uint64_t cut = 0;
+    // Collecting pays while a third of the row or less is collected; at a half it takes longer than not asking.
+    bool sparse = false;
     if (k != 0 && k <= kListed / 2) {
         // ---- few by count ----
         // The k-th largest of the threads' own maxima is at most the k-th largest of all, and hardly smaller while k is a
@@ -838,6 +840,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
         }
         cluster.sync();
         const uint32_t low_bin = sh.low_bin, high_bin = sh.high_bin, down_to = sh.found_count, low_before = sh.low_before;
+        sparse = down_to != 0 && down_to <= p.vocab / 3;
         if (down_to != 0 && down_to <= kListed) {
             // ---- few stay ----
             const float end = (float)(high_bin + 1);
@@ -901,7 +904,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             const float first = (float)low_bin, end = (float)(high_bin + 1), finer = (float)bins / (end - first);
             uint64_t above = 0;
             auto fine_bin = [&](float v) { return whole(fminf((v - first) * finer, last_bin)); };
-            slice.each_above(value_below(end), sh.queue[warp], [&](float x, uint32_t) {
+            auto add_fine = [&](float x, uint32_t) {
                 const float v = place_of(x, high, to_bin, last_bin);
                 if (v >= end) return;
                 const uint64_t w = weigh.of(x);
@@ -912,7 +915,9 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
                     atomicAdd(&sh.count[b], 1u);
                     atomicAdd(reinterpret_cast<unsigned long long *>(&sh.mass[b]), (unsigned long long)w);
                 }
-            });
+            };
+            if (sparse) slice.each_above(value_below(end), sh.queue[warp], add_fine);
+            else slice.each(add_fine);
             tell_parts(cluster, sh, 1, above);
             cluster.sync();
             const uint32_t fine_number = count_of(cluster, sh, bin);
@@ -933,7 +938,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             const uint32_t border = sh.fine_bin, border_count = sh.fine_count;
             const uint64_t before = sh.found_before;
             if (border_count != 0 && border_count <= kListed) {
-                gather<true>(cluster, sh, slice, value_below(end), [&](float x, uint32_t) {
+                gather<false>(cluster, sh, slice, value_below(end), [&](float x, uint32_t) {
                     const float v = place_of(x, high, to_bin, last_bin);
                     return v >= first && v < end && fine_bin(v) == border;
                 });
@@ -974,7 +979,7 @@ sample_kernel(const __grid_constant__ SampleArgs p, uint32_t slice_size) {
             if (lane < slice.tail) sum = kept(slice.at(slice.size - slice.tail + lane), slice.size - slice.tail + lane);
         } else {
             if (all && least == 0) slice.tile(t - 1, [&](float x, uint32_t) { sum += weigh.of(x); });
-            else if (all) slice.tile(t - 1, [&](float x, uint32_t i) { sum += kept(x, i); });
+            else if (all || !sparse) slice.tile(t - 1, [&](float x, uint32_t i) { sum += kept(x, i); });
             else slice.tile_above(t - 1, cut_logit, sh.queue[warp], [&](float x, uint32_t i) { sum += kept(x, i); });
         }
         sum = warp_sum(sum);
