@@ -1008,7 +1008,7 @@ int check_cache(const q4b_kv_cache *cache, const q4b_token_batch *batch, uint32_
     return Q4B_OK;
 }
 
-// [rows][stride] with `width` values used of every row: does [a, ...) touch [b, ...)?
+// [rows][stride] with `width` bytes used of every row.  Blocks of equal stride may be columns of one matrix.
 struct Block {
     const void *pointer;
     uint32_t rows;
@@ -1016,7 +1016,14 @@ struct Block {
     uintptr_t begin() const { return reinterpret_cast<uintptr_t>(pointer); }
     uintptr_t end() const { return begin() + (uintptr_t)((uint64_t)(rows - 1) * stride_bytes + width_bytes); }
 };
-bool overlap(const Block &a, const Block &b) { return a.begin() < b.end() && b.begin() < a.end(); }
+bool overlap(const Block &a, const Block &b) {
+    if (a.begin() >= b.end() || b.begin() >= a.end()) return false;
+    if (a.stride_bytes != b.stride_bytes) return true;
+    const uint64_t stride = a.stride_bytes;
+    const uint64_t ahead = b.begin() >= a.begin() ? (b.begin() - a.begin()) % stride
+                                                  : (stride - (a.begin() - b.begin()) % stride) % stride;
+    return ahead < a.width_bytes || ahead + b.width_bytes > stride;
+}
 
 }  // namespace
 
@@ -1059,9 +1066,9 @@ int q4b_rope_append(q4b_context *context, const q4b_kv_cache *cache, const q4b_t
     }
     const Block out_block = {q_out, batch->tokens, (uint64_t)ldq_out * 2, (uint64_t)q_heads * head * 2};
     const bool in_place = q == q_out && dtype == cache->dtype && q_head_stride == head && ldq == ldq_out;
-    if (!in_place && (overlap(out_block, {q, batch->tokens, ldq * item, q_width * item}) ||
-                      overlap(out_block, {k, batch->tokens, ldk * item, kv_width * item}) ||
-                      overlap(out_block, {v, batch->tokens, ldv * item, kv_width * item}))) {
+    if ((!in_place && overlap(out_block, {q, batch->tokens, ldq * item, q_width * item})) ||
+        overlap(out_block, {k, batch->tokens, ldk * item, kv_width * item}) ||
+        overlap(out_block, {v, batch->tokens, ldv * item, kv_width * item})) {
         set_error(error_message, error_capacity, "q_out overlaps q, k or v (only q itself with the same type and strides may be)");
         return Q4B_BAD_ARGUMENT;
     }

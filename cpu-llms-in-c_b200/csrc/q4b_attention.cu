@@ -10,7 +10,8 @@
 //     S^T [16 keys x 8 R rows] = K Q^T          (mma.sync m16n8k16, K from shared memory by ldmatrix)
 //     O^T [D x 8 R rows]      += V^T P^T        (V by ldmatrix.trans, P^T by movmatrix from S^T's registers)
 // in that orientation a row's maximum, sum and output column sit in the same lanes, eight rows cost no padding to
-// sixteen, and a warp needs nothing from the others until its share of the keys is done.
+// sixteen, and a warp needs nothing from the others until its share of the keys is done.  An fp16 weight has no bits below
+// 2^-24: with the largest at 1 a long context's many small ones would be lost together, so the largest is 2^15 there.
 //
 // Split: a unit is (sequence, key head, 8 R rows).  The units' groups of 16 keys form one list, cut into equal ranges,
 // one per thread block, whatever the lengths are (they live in device memory; the host does not know them).  Within
@@ -39,6 +40,8 @@ constexpr uint32_t kBlocksPerSm = 1;
 // a unit's share of a thread block is at least this many groups (one per warp): fewer would leave warps idle while
 // adding sums to join
 constexpr uint32_t kLeastShare = 8;
+// the largest weight, as a power of two
+template <typename T> constexpr float kLift = std::is_same<T, __half>::value ? 15.0f : 0.0f;
 constexpr uint32_t kCluster = 8;        // thread blocks of a cluster, where one sequence has the GPU to itself
 
 template <int D> struct Ring {
@@ -368,7 +371,7 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
                 for (int i = 0; i < 2; ++i) {
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) high[i] = fmaxf(high[i], __shfl_xor_sync(0xffffffffu, high[i], d));
-                    const float grown = fmaxf(top[r][i], high[i]);
+                    const float grown = fmaxf(top[r][i], high[i] - kLift<T>);
                     const float base = grown == -INFINITY ? 0.0f : grown;  // nothing visible so far
                     keep[r][i] = exp2_fast(top[r][i] - base);
                     top[r][i] = grown;

@@ -12,7 +12,8 @@ enum : uint32_t { kBadDescriptor = 0x1000u, kBadPage = kBadDescriptor | 1u, kBad
 
 __host__ __device__ inline void report(uint32_t *status, uint32_t code) {
 #ifdef __CUDA_ARCH__
-    atomicExch(status, code);
+    // an expired wait of queued work stays: q4b_sync has more to put right after one
+    if (*static_cast<volatile uint32_t *>(status) == 0) atomicExch(status, code);
 #else
     *status = code;  // the index arithmetic below is checked on the host too
 #endif

@@ -163,8 +163,8 @@ struct AttentionArgs {
     uint32_t most_tokens;
     float scale;
     uint32_t window, sinks;
-    float *partials;       // attention_workspace_bytes of scratch; its tail holds arrival counters, zero between launches
-    uint32_t *arrivals;
+    float *partials;       // attention_partial_bytes of scratch
+    uint32_t *arrivals;    // attention_arrival_bytes, zero between launches
     uint32_t *status;
 };
 // what every attention launch of a device may use: sums of split rows and their counters

@@ -289,7 +289,8 @@ typedef struct {
  * [tokens][ldq] with head h at h * q_head_stride (so a projection that interleaves q with something else is read in
  * place), k and v [tokens][ldk], [tokens][ldv] with heads next to each other; q, k and v share dtype (fp16, fp32 or
  * bf16) and may be columns of one matrix.  q_out is [tokens][ldq_out], heads next to each other; it may be q itself
- * when dtype, head stride and row stride agree, and must not overlap it otherwise.  Strides count values; pointers are
+ * when dtype, head stride and row stride agree; otherwise it must not overlap q, and never k or v (other columns
+ * of one matrix are no overlap).  Strides count values; pointers are
  * 16-byte aligned and strides whole multiples of 16 bytes.  Computed in fp32, rounded once.  A token whose place in
  * its sequence is negative (lengths[s] smaller than its rows: left padding) is skipped.  Two tokens of one call that
  * share a slot leave either one's values in it.  Asynchronous. */
@@ -302,7 +303,7 @@ int q4b_rope_append(q4b_context *context, const q4b_kv_cache *cache, const q4b_t
  * key[j][h / group]) value[j][h / group], group = q_heads / kv_heads.  q is [tokens][ldq], out [tokens][ldo], heads
  * next to each other, both in the cache's type; pointers 16-byte aligned, strides multiples of 8 values.  out must not
  * overlap q.  Scores, maxima, sums and the output's accumulation are fp32; a weight is rounded to the cache's type
- * before it meets the values.  A row that sees nothing (p < 0) is zeros.  What is not visible has no influence,
+ * before it meets the values (in fp16 to no less than 2^-35 of the largest one).  A row that sees nothing (p < 0) is zeros.  What is not visible has no influence,
  * whatever it holds, infinities and NaN included.  The result does not depend on timing.  The first call on a context
  * allocates a workspace (never while recording).  Asynchronous. */
 int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_token_batch *batch, const void *q,

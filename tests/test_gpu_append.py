@@ -208,5 +208,5 @@ def test_refusals(q4b, ctx):
         refused(rope)
     for change in ({"dtype": 7}, {"q_heads": 3}, {"q_ptr": d.ptr + 2}, {"k_ptr": 0}, {"ldq": 248}, {"ldq": 260},
                    {"q_head_stride": 32}, {"ldk": 120}, {"ldv": 132}, {"ldq_out": 248}, {"q_out_ptr": d.ptr + 16},
-                   {"q_out_ptr": d.ptr + 4096}, {"q_out_ptr": d.ptr, "ldq": 512}, {"dtype": q4b.F32, "q_out_ptr": d.ptr}):
+                   {"q_out_ptr": d.ptr + 4096}, {"q_out_ptr": d.ptr, "ldq": 512}, {"q_out_ptr": d.ptr, "k_ptr": d.ptr + 256}, {"dtype": q4b.F32, "q_out_ptr": d.ptr}):
         refused(**change)

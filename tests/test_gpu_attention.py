@@ -231,6 +231,97 @@ def test_a_recorded_call_follows_the_lengths(q4b, ctx):
             assert (np.abs(got - want) <= tolerance).all(), step
 
 
+@pytest.mark.parametrize("counts,lengths", [([1], [4000]), ([1, 1], [4000, 2000]), ([64], [4000])])
+def test_many_small_weights_of_fp16_are_not_lost(q4b, ctx, counts, lengths):
+    """One key far above 4,000 others whose weights are 2^-25 of its own: together they are a ten-thousandth of the sum, and
+    below the last bit that fp16 has next to 1.
+
+    Tolerance: that of attention_reference for what is as large as the answer; a weight's rounding is half an eps of
+    itself, or 2^-36 of the largest one's where that is more (fp16 ends at 2^-24; the largest is set to 2^11 or more)."""
+    rng = np.random.default_rng(21)
+    batch = Batch(rng, counts, lengths, 64, 1, 64, "f16")
+    batch.keys[:], batch.values[:] = 0.0, 1.0
+    for s in range(len(counts)):
+        page, place = batch.slot(s, 5)
+        batch.keys[page, 0, place, 0] = 1.0
+        batch.values[page, 0, place] = 0.0
+    q = np.zeros((batch.tokens, 2, 64), np.float16)
+    q[:, :, 0] = 1.0
+    scale = 25.0 * math.log(2.0)
+    got = widen(attend(q4b, ctx, batch, q, 2, scale, 0, 0), "f16")
+    want, tolerance = attention_reference(batch, q, 2, scale, 0, 0)
+    tolerance = tolerance + max(lengths) * 2.0 ** -36
+    assert (want > 40 * tolerance).all()   # losing them would show
+    assert (np.abs(got - want) <= tolerance).all()
+
+
+def test_sequences_that_share_pages(q4b, ctx):
+    """A common beginning is held once; the same page may even stand in a table twice."""
+    rng = np.random.default_rng(22)
+    for counts in ([1, 2, 1], [40, 33, 1]):
+        batch = Batch(rng, counts, [130, 170, 90], 32, 2, 128, "bf16")
+        batch.table[1, :2] = batch.table[0, :2]
+        batch.table[2, :2] = batch.table[0, 1]
+        check(q4b, ctx, batch, 4)
+
+
+def test_the_output_beside_the_queries(q4b, ctx):
+    """q and out may be columns of one matrix."""
+    rng = np.random.default_rng(23)
+    for counts, lengths in (([1, 3], [40, 20]), ([50], [60])):
+        batch = Batch(rng, counts, lengths, 16, 1, 64, "f16")
+        cache, described = batch.upload(q4b, ctx)
+        q = narrow(rng.standard_normal((batch.tokens, 2, 64)), "f16")
+        rows = np.zeros((batch.tokens, 264), np.float16)
+        rows[:, :128], rows[:, 256:] = q.reshape(batch.tokens, 128), 3.0
+        d = ctx.to_device(rows)
+        ctx.attention(cache, described, d.ptr, 2, d.ptr + 256, 0.125, ldq=264, ldo=264)
+        after = d.download(np.float16, rows.shape)
+        want, tolerance = attention_reference(batch, q, 2, 0.125, 0, 0)
+        assert (np.abs(widen(after[:, 128:256], "f16").reshape(want.shape) - want) <= tolerance).all()
+        assert (after[:, :128] == rows[:, :128]).all() and (after[:, 256:] == 3.0).all()
+        with pytest.raises(q4b.Q4Error):
+            ctx.attention(cache, described, d.ptr, 2, d.ptr + 240, 0.125, ldq=264, ldo=264)
+        with pytest.raises(q4b.Q4Error):   # its last columns reach into the next row's queries
+            ctx.attention(cache, described, d.ptr, 2, d.ptr + 400, 0.125, ldq=264, ldo=264)
+
+
+def test_two_contexts_at_once(q4b):
+    """Each has its own stream and workspace; their calls run next to each other, from a host thread each."""
+    import threading
+    failures = []
+
+    def work(seed):
+        try:
+            with q4b.Q4Context(0) as own:
+                rng = np.random.default_rng(seed)
+                for counts, lengths in (([1], [6000]), ([1, 1, 3], [3000, 70, 900]), ([200], [500]), ([1], [3000])):
+                    check(q4b, own, Batch(rng, counts, lengths, 64, 2, 128, "f16"), 4, seed=seed)
+        except BaseException as error:  # noqa: BLE001 -- told to the test
+            failures.append(error)
+    threads = [threading.Thread(target=work, args=(seed,)) for seed in (31, 32)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
+
+
+@pytest.mark.parametrize("begin", [[0, 3, 2, 5], [0, 40, 10, 60], [0, 2, 900, 5], [7, 7, 90, 91]])
+def test_begins_that_fall_or_pass_the_rows_are_reported(q4b, ctx, begin):
+    rng = np.random.default_rng(24)
+    batch = Batch(rng, [30, 20, 10], [100, 50, 40], 16, 2, 64, "f16")
+    for most in (1, 40):
+        cache, described = batch.upload(q4b, ctx, most)
+        batch.d_begin.upload(np.asarray(begin, dtype=np.uint32))
+        d_q, d_out = ctx.to_device(np.zeros((batch.tokens, 4, 64), np.float16)), ctx.alloc(batch.tokens * 4 * 64 * 2)
+        ctx.attention(cache, described, d_q.ptr, 4, d_out.ptr, 0.1)
+        with pytest.raises(q4b.Q4Error) as refused:
+            ctx.sync()
+        assert refused.value.status == 1 and "token_begin" in refused.value.message
+        check(q4b, ctx, Batch(rng, [30, 20, 10], [100, 50, 40], 16, 2, 64, "f16"), 4)
+
+
 def test_bad_pages_are_reported_and_not_followed(q4b, ctx):
     rng = np.random.default_rng(12)
     for counts in ([1, 1], [90, 40]):
