@@ -7,8 +7,9 @@
 // encode_delta (:668-674) / encode_attention (:747-753) and the out-projection with
 // residual at their tails (:716-723, :788-795), with their batched forms
 // encode_prefill_gemm_f16 (:885-928) and encode_prefill_gemm_residual (:930-1001).
-// What sits between those matmuls (norms, the DeltaNet recurrence, attention) is not
-// part of this library; the caller runs it on the same stream.
+// What sits between those matmuls is not queued from here: the norm (q4b_rmsnorm), the
+// rotation with the cache store (q4b_rope_append) and attention (q4b_attention) are calls
+// of their own on the same stream, the DeltaNet recurrence is the caller's.
 //
 // A layer holds the row slice of each matrix that this rank owns (column-parallel
 // over `world` ranks, 16-row granular).  Every call writes its slice at its
