@@ -75,6 +75,32 @@ template <> __device__ inline uint32_t pack2<__nv_bfloat16>(float low, float hig
 }
 __device__ inline float wide(__half x) { return __half2float(x); }
 __device__ inline float wide(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ inline float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// two floats of neighbouring registers, for the instructions that take both
+__device__ inline uint64_t two(float low, float high) {
+    uint64_t both;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(both) : "f"(low), "f"(high));
+    return both;
+}
+__device__ inline float2 apart(uint64_t both) {
+    float2 x;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x.x), "=f"(x.y) : "l"(both));
+    return x;
+}
+__device__ inline uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ inline uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ inline void pair_barrier(uint32_t id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 // (token, query head of the group) of every `step`th row, without a division for each
@@ -468,7 +494,8 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     }
                     float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 64; ++i) most[i & 3] = fmaxf(most[i & 3], __uint_as_float(raw[i >> 5][i & 31]));
+                    for (int i = 0; i < 64; i += 2)
+                        most[i >> 1 & 3] = max3(most[i >> 1 & 3], __uint_as_float(raw[i >> 5][i & 31]), __uint_as_float(raw[i >> 5][i + 1 & 31]));
                     float high = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
                     pair_barrier(5 + quad);  // the other half has read what it was told last time
                     exchange[half * 128 + row] = high;
@@ -497,15 +524,19 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     }
                     const float minus = top == -INFINITY ? 0.0f : -top;
                     uint32_t weights[32];
-                    float sum[2] = {0.0f, 0.0f};
+                    const uint64_t factors = two(c, c), offsets = two(minus, minus);
+                    uint64_t sum[2] = {0, 0};
 #pragma unroll
                     for (int i = 0; i < 32; ++i) {
-                        const float x = exp2_of(fmaf(__uint_as_float(raw[i >> 4][(2 * i) & 31]), c, minus));
-                        const float y = exp2_of(fmaf(__uint_as_float(raw[i >> 4][(2 * i + 1) & 31]), c, minus));
-                        sum[i & 1] += x + y;
-                        weights[i] = pack2<T>(x, y);
+                        float2 x = apart(fma2(two(__uint_as_float(raw[i >> 4][(2 * i) & 31]), __uint_as_float(raw[i >> 4][(2 * i + 1) & 31])),
+                                              factors, offsets));
+                        x.x = exp2_of(x.x);
+                        x.y = exp2_of(x.y);
+                        sum[i & 1] = add2(sum[i & 1], two(x.x, x.y));
+                        weights[i] = pack2<T>(x.x, x.y);
                     }
-                    total += sum[0] + sum[1];
+                    const float2 sums = apart(add2(sum[0], sum[1]));
+                    total += sums.x + sums.y;
                     tc_store_32(s_columns + half * 32, weights);
                     tc_wait_store();
                     // O(j - 1) is complete long before P(j) is needed; every warp sees every round of its barrier
