@@ -294,10 +294,15 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             constexpr uint64_t k_desc = ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
             const uint64_t v_desc = ((uint64_t)((128u << p.v_shift) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
                                     ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-            auto at = [](uint32_t address) { return (uint64_t)((address >> 4) & 0x3fffu); };
+            // a descriptor takes the low 18 bits of an address: in a cluster those above name the thread block
+            auto at = [](uint32_t address) { return (uint64_t)((address & 0x3ffffu) >> 4); };
             const bool leader = tc_leader();
             const uint32_t to_s = __shfl_sync(0xffffffffu, tmem_s, 0), to_o = __shfl_sync(0xffffffffu, tmem_o, 0);
-            const uint32_t rows0 = tc_smem_u32(query);
+            const uint64_t rows0 = k_desc + at(tc_smem_u32(query));
+            uint32_t v_step[S::v_rows / 16];  // where a slot's steps of 16 values lie, in units of 16 bytes as descriptors count
+#pragma unroll
+            for (uint32_t k = 0; k < S::v_rows / 16; ++k)
+                v_step[k] = ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 8;
             uint32_t k_slot = 0, k_lap = 0, v_slot = 0, v_lap = 0, looked = 0, begun = 0;
             auto advance = [](uint32_t &slot, uint32_t &lap) {
                 if (++slot == S::slots) {
@@ -310,10 +315,10 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 for (uint32_t part = 0; part < S::parts; ++part) {
                     if (!tc_warp_wait(k_full0 + 8 * k_slot, k_lap & 1)) return false;
                     tc_fence_after();
-                    const uint32_t keys = k_ring + k_slot * kSlotBytes, rows = rows0 + part * (kTileRowsQ * 128);
+                    const uint64_t keys = k_desc + at(k_ring + k_slot * kSlotBytes), rows = rows0 + part * (kTileRowsQ * 128 >> 4);
 #pragma unroll
                     for (uint32_t k = 0; k < 4; ++k)
-                        tc_mma_shared_by(leader, to_s + (j & 1) * 128, k_desc | at(rows + k * 32), k_desc | at(keys + k * 32), s_idesc,
+                        tc_mma_shared_by(leader, to_s + (j & 1) * 128, rows + k * 2, keys + k * 2, s_idesc,
                                          part > 0 || k > 0 ? 1u : 0u);
                     tc_commit_by(leader, k_empty0 + 8 * k_slot);
                     advance(k_slot, k_lap);
@@ -326,19 +331,20 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             if (ok) ok = scores(0);
             if (ok && n > 1) ok = scores(1);
             for (uint32_t j = 0; j < n && ok; ++j) {
+                // the values came long ago: their waits (100 clocks each) are over before the weights are there
+                uint32_t slot = v_slot, lap = v_lap;
+#pragma unroll
+                for (uint32_t part = 0; part < S::parts; ++part) {
+                    if (ok) ok = tc_warp_wait(v_full0 + 8 * slot, lap & 1);
+                    advance(slot, lap);
+                }
+                if (!ok) break;
                 // a masked tile's values are handed to the warp that looks at them and handed back: a strict exchange,
                 // so neither side can miss a round of a barrier that the other is already past
                 const bool edge = !u.clear(a, u.key(j));
                 uint32_t steps = 0xffu;  // of 16 keys that some row sees
                 if (edge) {
                     steps = __ballot_sync(0xffffffffu, lane < kTileKeys / 16 && u.any(a, u.key(j) + lane * 16, 16));
-                    uint32_t slot = v_slot, lap = v_lap;
-#pragma unroll
-                    for (uint32_t part = 0; part < S::parts; ++part) {
-                        if (ok) ok = tc_warp_wait(v_full0 + 8 * slot, lap & 1);
-                        advance(slot, lap);
-                    }
-                    if (!ok) break;
                     if (leader) tc_mbar_arrive(v_look);
                 }
                 ok = tc_warp_wait(p_full0 + 8 * (j & 1), (j >> 1) & 1);
@@ -346,26 +352,31 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     ok = tc_warp_wait(v_ready, looked & 1);
                     ++looked;
                 }
+                if (!ok) break;
                 tc_fence_after();
+                const uint32_t weights = to_s + (j & 1) * 128;
 #pragma unroll
                 for (uint32_t part = 0; part < S::parts; ++part) {
-                    if (ok) ok = tc_warp_wait(v_full0 + 8 * v_slot, v_lap & 1);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint32_t values = v_ring + v_slot * kSlotBytes;
+                    constexpr uint32_t kSteps = S::v_rows / 16;
+                    const uint64_t values = v_desc + at(v_ring + v_slot * kSlotBytes);
+                    if (steps == 0xffu) {
 #pragma unroll
-                    for (uint32_t k = 0; k < S::v_rows / 16; ++k) {
-                        // keys that no row sees are left out, with whatever their place in the slot holds
-                        if (!(steps >> (part * (S::v_rows / 16) + k) & 1u)) continue;
-                        tc_mma_by(leader, to_o, to_s + (j & 1) * 128 + (part * (S::v_rows / 16) + k) * 8,
-                                  v_desc | at(values + ((k * 16 >> p.v_shift << p.v_shift) * S::parts + (k * 16 & ((1u << p.v_shift) - 1))) * 128),
-                                  o_idesc, begun);
-                        begun = 1;
+                        for (uint32_t k = 0; k < kSteps; ++k)
+                            tc_mma_by(leader, to_o, weights + (part * kSteps + k) * 8, values + v_step[k], o_idesc,
+                                      part > 0 || k > 0 ? 1u : begun);
+                    } else {
+#pragma unroll
+                        for (uint32_t k = 0; k < kSteps; ++k) {
+                            // keys that no row sees are left out, with whatever their place in the slot holds
+                            if (!(steps >> (part * kSteps + k) & 1u)) continue;
+                            tc_mma_by(leader, to_o, weights + (part * kSteps + k) * 8, values + v_step[k], o_idesc, begun);
+                            begun = 1;
+                        }
                     }
                     tc_commit_by(leader, v_empty0 + 8 * v_slot);
                     advance(v_slot, v_lap);
                 }
-                if (!ok) break;
+                begun = 1;
                 tc_commit_by(leader, o_done);
                 if (j + 2 < n) ok = scores(j + 2);
             }

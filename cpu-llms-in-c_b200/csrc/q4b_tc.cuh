@@ -86,7 +86,6 @@ __device__ inline void tc_load_16(uint32_t address, uint32_t (&r)[16]) {
         : "r"(address));
 }
 
-// cuTensorMapEncodeTiled through the runtime, so the library links libcudart only
 __device__ inline void tc_load_32(uint32_t address, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
@@ -153,6 +152,7 @@ __device__ inline void tc_tensor_copy_3d_by(bool leader, uint32_t destination, c
         : "memory");
 }
 
+// cuTensorMapEncodeTiled through the runtime, so the library links libcudart only
 typedef CUresult (*EncodeTiledFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
