@@ -12,7 +12,11 @@
 // the rest, half a turn at most.  One thread does that per (token, pair); the heads share it through shared memory.
 //
 // Work unit: 16 values of one head -- 8 + 8 that are partners in the HALVES form, 16 neighbours otherwise -- so a
-// thread reads both partners before it writes either and q may be turned in place.
+// thread reads both partners before it writes either and q may be turned in place.  Two units per thread at once took
+// longer (57 us against 52 us for 8,192 tokens).
+//
+// Measured on B200 (24 query heads and 4 key heads of 256, 16-bit in and out): 8,192 tokens in 52 us = 5.2 TB/s of 6.54, one
+// token in 4.1 us on the device, 6.4 us with the host's call.
 #include "q4b_cache.cuh"
 
 namespace q4b {

@@ -25,6 +25,12 @@
 //
 // When there are fewer units than SMs the keys of a unit are split over a cluster of 2 to 8 thread blocks, whose sums meet
 // in distributed shared memory.
+//
+// What bounds it: keys and values from L2, 512 D bytes per tile and SM.  At D = 256 the ring holds 1.25 tiles and 42 bytes
+// per clock and SM arrive (more than 10 TB/s over the chip); a tile takes some 3,000 clocks, 2,048 of them products.
+// Measured on B200 (fp16 and bf16 alike): a prompt of 8,192 tokens, 24 query heads on 4 key heads of 256, 720 us = 1,145
+// TFLOP/s of 1,677; four prompts of up to 4,001 tokens behind a window of 1,024, 437 us; 511 tokens behind 30,001, 16 heads
+// on 4 of 128, 154 us = 822 TFLOP/s; four tokens of six users behind a window of 4,096, 31.4 us.
 #include "q4b_cache.cuh"
 #include "q4b_tc.cuh"
 
