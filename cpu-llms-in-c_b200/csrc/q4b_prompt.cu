@@ -250,7 +250,8 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             const uint32_t wanted = __ballot_sync(0xffffffffu, (lane << shift) < kTileKeys && u.key(j) + my_token < keys_end &&
                                                                    u.any(a, u.key(j) + my_token, 1u << shift));
             if (page >= a.cache.pages) {  // never followed: the pool's first page stands in for it
-                report(a.status, kBadPage);
+                // the entry of a box that is not fetched may be anything: pages behind a window are dealt anew
+                if (wanted >> lane & 1u) report(a.status, kBadPage);
                 page = 0;
             }
             const int line = (int)((page * a.cache.kv_heads + u.head) * a.cache.page_tokens + (token & (a.cache.page_tokens - 1)));
