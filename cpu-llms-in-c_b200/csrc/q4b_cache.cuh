@@ -10,12 +10,13 @@ namespace q4b {
 enum : uint32_t { kBadDescriptor = 0x1000u, kBadPage = kBadDescriptor | 1u, kBadLength = kBadDescriptor | 2u,
                   kBadBegin = kBadDescriptor | 3u };
 
+// Only a word that holds nothing is written: the code of an expired wait stays (q4b_sync has more to put right after
+// one), however close behind it the descriptor's comes.
 __host__ __device__ inline void report(uint32_t *status, uint32_t code) {
 #ifdef __CUDA_ARCH__
-    // an expired wait of queued work stays: q4b_sync has more to put right after one
-    if (*static_cast<volatile uint32_t *>(status) == 0) atomicExch(status, code);
+    atomicCAS(status, 0u, code);
 #else
-    *status = code;  // the index arithmetic below is checked on the host too
+    if (*status == 0) *status = code;  // the index arithmetic below is checked on the host too
 #endif
 }
 
