@@ -107,6 +107,11 @@ append_kernel(const __grid_constant__ AppendArgs p) {
             sincospif((float)(2.0 * (turns - rint(turns))), &sine, &cosine);
             turn[warp][i] = make_float2(cosine, sine);
         }
+    } else if (warp >= kAppendTokens) {
+        // the warps without a token look at all sequences: rows that a wrong begin leaves to nobody are told as well
+        constexpr uint32_t kLookers = kAppendThreads - 32 * kAppendTokens;
+        for (uint32_t s = blockIdx.x * kLookers + threadIdx.x - 32 * kAppendTokens; s < p.batch.sequences; s += gridDim.x * kLookers)
+            sequence_rows(p.batch, p.cache.page_tokens, s, p.status);
     }
     __syncthreads();
     const uint32_t per_head = D / 16, heads = p.q_heads + 2 * p.cache.kv_heads;

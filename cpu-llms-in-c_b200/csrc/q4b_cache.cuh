@@ -24,7 +24,8 @@ __host__ __device__ inline void report(uint32_t *status, uint32_t code) {
 struct SequenceRows {
     uint32_t begin, count, length;
 };
-// The descriptor's numbers held to what the buffers have, whatever they say.
+// The descriptor's numbers held to what the buffers have, whatever they say.  The length of a sequence that brings no token
+// is used for nothing and may be anything.
 __host__ __device__ inline SequenceRows sequence_rows(const BatchView &batch, uint32_t page_tokens, uint32_t s, uint32_t *status) {
     SequenceRows rows;
     const uint32_t from = batch.begin[s], to = batch.begin[s + 1];
@@ -35,7 +36,7 @@ __host__ __device__ inline SequenceRows sequence_rows(const BatchView &batch, ui
     const uint64_t room = (uint64_t)batch.table_stride * page_tokens;
     rows.length = batch.lengths[s];
     if (rows.length > room || rows.length > 0x7fffffffu) {
-        report(status, kBadLength);
+        if (rows.count != 0) report(status, kBadLength);
         rows.length = room < 0x7fffffffu ? (uint32_t)room : 0x7fffffffu;
     }
     return rows;

@@ -171,7 +171,8 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
         const uint32_t tile = index / a.cache.kv_heads;
         uint32_t before = 0;
         bool found = false;
-        for (uint32_t s0 = 0; s0 < a.batch.sequences && !found; s0 += 32) {
+        // the first block looks at the sequences behind its own too: somebody has to tell of each one's mistakes
+        for (uint32_t s0 = 0; s0 < a.batch.sequences && (!found || blockIdx.x == 0); s0 += 32) {
             uint32_t own = 0;
             if (s0 + lane < a.batch.sequences)
                 own = ceil_div(sequence_rows(a.batch, a.cache.page_tokens, s0 + lane, a.status).count * a.group, kTileRowsQ);
@@ -182,7 +183,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 if (lane >= (uint32_t)d) inclusive += y;
             }
             const uint32_t passed = __ballot_sync(0xffffffffu, before + inclusive > tile);
-            if (passed != 0) {
+            if (passed != 0 && !found) {
                 const int at = __ffs(passed) - 1;
                 u.sequence = s0 + at;
                 u.row0 = (tile - before - __shfl_sync(0xffffffffu, inclusive - own, at)) * kTileRowsQ;

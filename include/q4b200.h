@@ -260,8 +260,9 @@ int q4b_matmul_rows(q4b_context *context, const q4b_weight *weight, const uint32
  *
  * What the device finds wrong in them (a page that the pool does not have, a table too short for a length,
  * token_begin that falls or passes `tokens`) is skipped, never followed, and reported by the next q4b_sync with
- * status 1; the outputs of that call are then not to be used.  Entries of pages that no new token sees or writes
- * (in front of a window and behind the sinks) may hold anything: such pages can be given to others. */
+ * status 1; the outputs of that call are then not to be used.  The length of a sequence that brings no token is not
+ * looked at.  Entries of pages that no new token sees or writes (in front of a window and behind the sinks) may hold
+ * anything: such pages can be given to others. */
 typedef struct {
     void *keys, *values;
     int dtype; /* Q4B_F16 or Q4B_BF16 */
