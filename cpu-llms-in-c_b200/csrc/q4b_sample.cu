@@ -248,12 +248,15 @@ struct Slice {
 struct Weigh {
     const uint2 *power;
     float high, rate, rate_low;  // log2(e) / temperature = rate + rate_low; all finite
+    float shrink;                // 1, or less where the largest logit is infinite
     __device__ inline void set(float largest, float temperature) {
         const double exact = 1.4426950408889634074 / (double)temperature;
         high = largest;
+        shrink = 1.0f;
         rate = fminf((float)exact, 3.0e38f);
         rate_low = rate < 3.0e38f ? (float)(exact - (double)rate) : 0.0f;
-        if (largest == INFINITY) {  // its equals share everything: they become the largest number, everything else is far away
+        if (largest == INFINITY) {  // its equals share everything: they become the largest number, all else is halved and far away
+            shrink = 0.5f;
             high = 3.402823466e38f;
             rate = 1.0f;
             rate_low = 0.0f;
@@ -276,7 +279,7 @@ struct Weigh {
     }
     __device__ inline uint64_t of(float x) const {
         float own;  // at most the largest (an infinity), a NaN stays one
-        asm("min.NaN.f32 %0, %1, %2;" : "=f"(own) : "f"(x), "f"(high));
+        asm("min.NaN.f32 %0, %1, %2;" : "=f"(own) : "f"(x * shrink), "f"(high));
         const float d = high - own;
         // d + low = high - x exactly, for 16-bit logits too: next to a large one a tiny one's bits end up beyond fp32's, and
         // leaving them out (2^-22 of a weight) saves 0.6 us of 95 for 33 rows

@@ -323,8 +323,9 @@ int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_tok
  * A NaN in temperature is greedy, one in top_p or min_p is off, one in uniform is 0.
  * The token is the first one, in index order, at which the running sum of the kept weights exceeds uniform[row] (in
  * [0, 1)) times their sum.  tokens [rows] and, if not NULL, probabilities [rows] (the token's share among the kept)
- * are written.  A NaN logit counts as -infinity; several logits of +infinity share everything; a row with nothing above
- * -infinity gives token 0xffffffff and probability 0.  Sums are exact integers of weights in units of 2^-42, so a
+ * are written.  A NaN logit counts as -infinity; several logits of +infinity share everything; a logit further below the
+ * largest than fp32's largest number has no weight at any temperature; a row with nothing above -infinity gives token
+ * 0xffffffff and probability 0.  Sums are exact integers of weights in units of 2^-42, so a
  * result depends on nothing but its row.  vocab is 1 .. 2^20; logits are aligned to their type.  Asynchronous. */
 typedef struct {
     const float *temperature;

@@ -43,3 +43,24 @@ def test_tiny_logits_beside_a_large_one(q4b, ctx, dtype, high, tiny, temperature
         off = probability * (2.0 ** -24 + 2.0 ** -28 + vocab * 2.0 ** -43) + 2.0 ** -43 / total
         assert tokens[r] == want and abs(share[r] - probability) <= off, (share[r], probability, off)
     assert small
+
+
+@pytest.mark.parametrize("dtype,largest", [("f32", 3.4028234663852886e38), ("bf16", 3.3895313892515355e38), ("f16", 65504.0)])
+@pytest.mark.parametrize("vocab", [40, 9000, 50_000])
+def test_the_largest_finite_logit_beside_infinities(q4b, ctx, dtype, largest, vocab):
+    """Logits of +infinity share everything: nothing is left for a finite one, however large."""
+    rng = np.random.default_rng(vocab)
+    logits = rng.standard_normal((4, vocab))
+    places = np.sort(rng.choice(np.arange(4, vocab), size=4, replace=False))
+    logits[:, places] = np.inf
+    logits[:, [0, 2, vocab - 1]] = largest
+    logits[:, 3] = -largest
+    logits[:, 1] = np.nan
+    if vocab - 1 in places:
+        logits[:, vocab - 1] = np.inf
+    u = [0.0, 0.3, 0.6, 0.99]
+    want = places[[0, 1, 2, 3]]
+    for rules in ({}, {"temperature": [0.01, 1.0, 100.0, 1e30]}, {"top_k": [6] * 4}, {"top_p": [0.999] * 4},
+                  {"min_p": [1e-6] * 4}, {"top_k": [vocab - 1] * 4, "top_p": [0.99] * 4, "min_p": [0.5] * 4}):
+        tokens, share, _ = run(q4b, ctx, logits, dtype, u, rules)
+        assert list(tokens) == list(want) and (share == 0.25).all(), (rules, tokens, share)
