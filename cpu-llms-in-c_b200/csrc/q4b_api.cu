@@ -1110,8 +1110,8 @@ int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_tok
     AttentionArgs args = {};
     code = check_cache(cache, batch, q_heads, &args.cache, &args.batch, error_message, error_capacity);
     if (code != Q4B_OK) return code;
-    if (!std::isfinite(scale)) {
-        set_error(error_message, error_capacity, "scale is not finite");
+    if (!std::isfinite(scale * 1.44269504088896341f)) {  // the kernels count in powers of two
+        set_error(error_message, error_capacity, "scale x log2(e) is not finite in fp32");
         return Q4B_BAD_ARGUMENT;
     }
     if (batch->tokens == 0 || batch->sequences == 0) return Q4B_OK;

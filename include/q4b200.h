@@ -303,12 +303,12 @@ int q4b_rope_append(q4b_context *context, const q4b_kv_cache *cache, const q4b_t
 /* Causal attention of the batch's tokens over the cache: a token at place p sees the cached tokens j <= p, with a
  * window (window > 0) only those with j > p - window or j < sinks.  out[row][h] = sum_j softmax_j(scale * q[row][h] .
  * key[j][h / group]) value[j][h / group], group = q_heads / kv_heads.  q is [tokens][ldq], out [tokens][ldo], heads
- * next to each other, both in the cache's type; pointers 16-byte aligned, strides multiples of 8 values.  out must not
- * overlap q.  Scores, maxima, sums and the output's accumulation are fp32; a weight is rounded to the cache's type
- * before it meets the values and the sum (in fp16 to steps of 2^-31 of the largest one where those are coarser), so that
- * equal values come back as they are, to fp32's accuracy.  A row that sees nothing (p < 0) is zeros.  What is not visible
- * has no influence, whatever it holds, infinities and NaN included.  The result does not depend on timing.  The first
- * call on a context allocates a workspace (never while recording).  Asynchronous. */
+ * next to each other, both in the cache's type; pointers 16-byte aligned, strides multiples of 8 values; scale x log2(e)
+ * is finite in fp32.  out must not overlap q.  Scores, maxima, sums and the output's accumulation are fp32; a weight is
+ * rounded to the cache's type before it meets the values and the sum (in fp16 to steps of 2^-31 of the largest one where
+ * those are coarser), so that equal values come back as they are, to fp32's accuracy.  A row that sees nothing (p < 0) is
+ * zeros.  What is not visible has no influence, whatever it holds, infinities and NaN included.  The result does not
+ * depend on timing.  The first call on a context allocates a workspace (never while recording).  Asynchronous. */
 int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_token_batch *batch, const void *q,
                   uint32_t ldq, uint32_t q_heads, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
                   char *error_message, size_t error_capacity);
