@@ -849,7 +849,8 @@ cudaError_t launch_prompt_head(const AttentionArgs &args, int sm_count, cudaStre
 }  // namespace
 
 bool prompt_serves(const AttentionArgs &args) {
-    // TMA counts the pools' rows in 31 bits
+    // TMA counts the pools' rows in 31 bits.  No B200 holds such a pool (256 GiB at 64 values a row); a cache that declares
+    // more pages than it uses may count as one, and is served as before, by the other kernel
     return (uint64_t)args.cache.pages * args.cache.kv_heads * args.cache.page_tokens <= 0x7fffffffull;
 }
 
