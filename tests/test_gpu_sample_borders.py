@@ -41,7 +41,7 @@ def test_tiny_logits_beside_a_large_one(q4b, ctx, dtype, high, tiny, temperature
         assert margin > 2.0 ** -28 + vocab * 2.0 ** -42   # nowhere near a border: the token is determined
         small += want != 5
         off = probability * (2.0 ** -24 + 2.0 ** -28 + vocab * 2.0 ** -43) + 2.0 ** -43 / total
-        assert tokens[r] == want and abs(share[r] - probability) <= off, (share[r], probability, off)
+        assert tokens[r] == want and abs(float(share[r]) - probability) <= off, (share[r], probability, off)
     assert small
 
 
@@ -118,4 +118,4 @@ def test_deep_cuts_of_long_rows(q4b, ctx, dtype, vocab, rules):
         assert len(may) < 64   # of tens of thousands
         assert int(tokens[r]) in may, (r, tokens[r], may)
         want = may[int(tokens[r])]
-        assert abs(share[r] - want) <= want * (2.0 ** -24 + 2.0 ** -28 + 2 * doubt) + 2.0 ** -42, (r, share[r], want)
+        assert abs(float(share[r]) - want) <= want * (2.0 ** -24 + 2.0 ** -28 + 2 * doubt) + 2.0 ** -42, (r, share[r], want)
