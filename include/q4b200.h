@@ -245,7 +245,9 @@ int q4b_matmul_rows(q4b_context *context, const q4b_weight *weight, const uint32
                     char *error_message, size_t error_capacity);
 /* ---- between a layer's projections: the paged cache and attention over it (the place of the rotation, cache
  * store and GQA decode kernels that the reference encodes between encode_attention's two projections,
- * qwen38_m3_decode.m:747-795; the paged form, ragged batches, windows and sinks have no counterpart there).
+ * qwen38_m3_decode.m:747-795; the paged form, ragged batches, windows and sinks have no counterpart there).  What a
+ * model does to q and k in front of the rotation (the RMS norm of each head, whose weights an attention layer's image
+ * holds) and to the output behind attention (its gate) is not part of these calls: the caller runs it on the same stream.
  *
  * q4b_kv_cache names one layer's cache: two pools of pages in DEVICE memory, each [pages][kv_heads][page_tokens]
  * [head_size], fp16 or bf16, 16-byte aligned.  page_tokens is a power of two from 16 to 1024, head_size 64, 128
@@ -307,8 +309,10 @@ int q4b_rope_append(q4b_context *context, const q4b_kv_cache *cache, const q4b_t
  * is finite in fp32.  out must not overlap q.  Scores, maxima, sums and the output's accumulation are fp32; a weight is
  * rounded to the cache's type before it meets the values and the sum (in fp16 to steps of 2^-31 of the largest one where
  * those are coarser), so that equal values come back as they are, to fp32's accuracy.  A row that sees nothing (p < 0) is
- * zeros.  What is not visible has no influence, whatever it holds, infinities and NaN included.  The result does not
- * depend on timing.  The first call on a context allocates a workspace (never while recording).  Asynchronous. */
+ * zeros.  What is not visible has no influence, whatever it holds, infinities and NaN included; in calls of many rows
+ * per sequence a value of that kind which some rows see and others do not has its keys gone through one by one: right,
+ * but orders of magnitude slower.  The result does not depend on timing.  The first call on a context allocates a
+ * workspace (never while recording).  Asynchronous. */
 int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_token_batch *batch, const void *q,
                   uint32_t ldq, uint32_t q_heads, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
                   char *error_message, size_t error_capacity);
@@ -653,7 +657,8 @@ int q4b_probe_signal(q4b_context *context, void *own_words, void *peer_words, ui
 
 /* ---- replay of a recorded call sequence (one command buffer per token in the
  * reference, qwen38_m3_decode.m:1614-1690): calls between begin and end are
- * captured instead of executed. */
+ * captured instead of executed.  A recorded call keeps the workspaces of the context it
+ * was recorded on: launch it on that one. */
 int q4b_graph_begin(q4b_context *context, char *error_message, size_t error_capacity);
 int q4b_graph_end(q4b_context *context, q4b_graph **graph, char *error_message,
                   size_t error_capacity);
