@@ -50,3 +50,43 @@ def test_a_cache_declared_with_more_rows_than_the_copies_count(q4b, ctx, head, g
         ctx.sync()
         got = widen(d_out.download(np.uint16, q.shape), "bf16")
         assert (np.abs(got - want) <= tolerance).all(), pages
+
+
+@pytest.mark.parametrize("head,page", [(256, 16), (64, 128)])
+def test_pages_far_behind_the_pools_start(q4b, ctx, head, page):
+    """Pools of 9 GB: the last pages begin beyond 2^32 values.  Written and read there, a cache gives the same bits as a small
+    one."""
+    rng = np.random.default_rng(page)
+    kv_heads, group, length = 2, 6, 2 * page + 5
+    far = 9 * 2 ** 30 // (2 * page * kv_heads * head)
+    assert (far - 3) * page * kv_heads * head > 2 ** 32
+    x = {name: narrow(rng.standard_normal((length, heads * head)), "bf16") for name, heads in
+         (("q", kv_heads * group), ("k", kv_heads), ("v", kv_heads))}
+    d = {name: ctx.to_device(bits) for name, bits in x.items()}
+    begin, lengths = ctx.to_device(np.array([0, length], np.uint32)), ctx.to_device(np.array([length], np.uint32))
+    one = ctx.to_device(np.array([0, 1], np.uint32))
+    answers = []
+    for pages in (3, far):
+        pools = [ctx.alloc(pages * page * kv_heads * head * 2) for _ in range(2)]
+        table = ctx.to_device(np.array([pages - 1, pages - 3, pages - 2], np.uint32))
+        cache = q4b.KVCache(keys=pools[0].ptr, values=pools[1].ptr, dtype=q4b.BF16, pages=pages, page_tokens=page, kv_heads=kv_heads,
+                            head_size=head)
+        batch = q4b.TokenBatch(sequences=1, tokens=length, most_tokens=length, token_begin=begin.ptr, lengths=lengths.ptr,
+                               page_table=table.ptr, table_stride=3)
+        turned = ctx.alloc(x["q"].nbytes)
+        ctx.rope_append(cache, batch, q4b.Rope(rotary_size=head, pairing=q4b.ROPE_HALVES, base=1e4), d["q"].ptr, d["k"].ptr, d["v"].ptr,
+                        q4b.BF16, kv_heads * group, turned.ptr)
+        prompt, single = ctx.alloc(x["q"].nbytes), ctx.alloc(x["q"].nbytes // length)
+        ctx.attention(cache, batch, turned.ptr, kv_heads * group, prompt.ptr, 0.1)
+        last = q4b.TokenBatch(sequences=1, tokens=1, most_tokens=1, token_begin=one.ptr, lengths=lengths.ptr, page_table=table.ptr,
+                              table_stride=3)
+        ctx.attention(cache, last, turned.ptr + (length - 1) * kv_heads * group * head * 2, kv_heads * group, single.ptr, 0.1)
+        ctx.sync()
+        answers.append((turned.download(np.uint16, x["q"].shape), prompt.download(np.uint16, x["q"].shape),
+                        single.download(np.uint16, (kv_heads * group * head,))))
+        for pool in pools:
+            pool.free()
+    for near, away in zip(*answers):
+        assert (near == away).all()
+    tolerance = 2.0 ** -7 * np.abs(widen(answers[0][1][-1], "bf16")).max()   # two kernels' roundings of one row
+    assert (np.abs(widen(answers[0][1][-1], "bf16") - widen(answers[0][2], "bf16")) <= tolerance).all()
