@@ -28,7 +28,7 @@
 // left for units that take several clusters.
 //
 // Measured on B200 (24 query heads on 4 key heads of 256): single tokens of 32 users with 4,000 to 16,384 cached ones each,
-// bf16, 218 us = 6.3 TB/s of 6.54; one token behind 1,024, 10.7 us, which is latency: lengths, page number, keys, exchange.
+// bf16, 218 us = 6.3 TB/s of 6.54; one token behind 1,024, 11 us, which is latency: lengths, page number, keys, exchange.
 #include "q4b_cache.cuh"
 
 #include <cooperative_groups.h>

@@ -7,7 +7,7 @@
 //
 // A row is spread over a cluster of 1 to 8 thread blocks.  Few rows are kept in shared memory after their one trip from
 // HBM; with many rows in flight the passes read them again from L2 instead, which leaves room for two thread blocks
-// per SM whose passes hide each other's waits (256 rows of 248,320 fp32 logits: 188 us against 282 us on chip; 18 rows the
+// per SM whose passes hide each other's waits (256 rows of 248,320 fp32 logits: 190 us against 282 us on chip; 18 rows the
 // other way, 31 us on chip against 35 us, with top-p 72 us against 80 us).
 //   extremes  the largest and the smallest finite logit (greedy ends here)
 //   counts    2048 bins, linear in the distance to the largest logit: linear bins spread a row evenly, where bins of
@@ -27,8 +27,9 @@
 // for the rest.  In fp64 the same pass is bound by the fp64 pipe and takes twice as long.
 //
 // Measured on B200 (248,320 logits a row): one fp32 row 10 us when greedy, 18 us with a top-k below 200, 29 to 61 us without
-// one; 33 fp16 rows by top-p 95 us; 256 fp32 rows, the whole distribution, 188 us = 1.35 TB/s, bound by the weights'
-// instructions (62% of the issue slots are taken).
+// one; 33 fp16 rows by top-p 95 us; 256 fp32 rows, the whole distribution, 190 us = 1.34 TB/s.  No unit is full in either of
+// the last two: 55 instructions per logit take 58% of the issue slots (ALU 46%, FMA 26%, DRAM 18%) and waits for loads and
+// barriers show at 43% of the warps; by top-p 134 instructions per logit take 51%, and barriers between a row's phases most.
 #include "q4b_kernels.h"
 
 #include <cooperative_groups.h>
