@@ -109,9 +109,11 @@ append_kernel(const __grid_constant__ AppendArgs p) {
         }
     } else if (warp >= kAppendTokens) {
         // the warps without a token look at all sequences: rows that a wrong begin leaves to nobody are told as well
+        // (in 64 bits: the grid's threads are more than 2^32 from 2^27 rows on)
         constexpr uint32_t kLookers = kAppendThreads - 32 * kAppendTokens;
-        for (uint32_t s = blockIdx.x * kLookers + threadIdx.x - 32 * kAppendTokens; s < p.batch.sequences; s += gridDim.x * kLookers)
-            sequence_rows(p.batch, p.cache.page_tokens, s, p.status);
+        for (uint64_t s = (uint64_t)blockIdx.x * kLookers + threadIdx.x - 32 * kAppendTokens; s < p.batch.sequences;
+             s += (uint64_t)gridDim.x * kLookers)
+            sequence_rows(p.batch, p.cache.page_tokens, (uint32_t)s, p.status);
     }
     __syncthreads();
     const uint32_t per_head = D / 16, heads = p.q_heads + 2 * p.cache.kv_heads;
