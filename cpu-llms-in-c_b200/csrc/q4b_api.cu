@@ -37,7 +37,7 @@ struct q4b_context {
     float *tc_workspace;      // partial tiles of the tensor-core GEMM when it splits tiles over CTAs
     size_t tc_workspace_bytes;
     uint32_t *tc_flags;
-    float *attention_partials;     // sums of query rows whose keys are split over thread blocks
+    float *attention_partials;     // sums of query rows whose keys are split over thread blocks, then folded sums of long ones
     uint32_t *attention_arrivals;  // their counters, zero between launches
 };
 
@@ -1139,7 +1139,8 @@ int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_tok
         uint32_t *arrivals = nullptr;
         cudaError_t status = context->attention_partials != nullptr
                                  ? cudaSuccess
-                                 : cudaMalloc(&context->attention_partials, attention_partial_bytes(context->sm_count));
+                                 : cudaMalloc(&context->attention_partials, attention_partial_bytes(context->sm_count) +
+                                                                                attention_fold_bytes(context->sm_count));
         if (status == cudaSuccess) status = cudaMalloc(&arrivals, arrival_bytes);
         if (status == cudaSuccess) status = cudaMemsetAsync(arrivals, 0, arrival_bytes, context->stream);
         if (status != cudaSuccess) {
@@ -1159,6 +1160,7 @@ int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_tok
     args.window = window;
     args.sinks = sinks;
     args.partials = context->attention_partials;
+    args.folds = context->attention_partials + attention_partial_bytes(context->sm_count) / sizeof(float);
     args.arrivals = context->attention_arrivals;
     args.status = context->status_device;
     cudaError_t status = launch_attention(args, context->sm_count, context->stream);

@@ -23,6 +23,10 @@
 // the end of a unit the warps' sums meet in shared memory.  A unit that is cut over thread blocks leaves fp32 sums in
 // the workspace; whoever arrives last adds them up in block order, so results do not depend on timing.
 //
+// Matrix instructions cut a running sum off where they would have to round it, so a long chain of them comes out too small
+// (by 8 x 10^-4 over the 8,192 products of a warp at a million keys).  A thread block's range of a unit is therefore taken in
+// pieces of at most 8 x 512 groups (fp16; 8 x 4,096 in bf16), whose sums meet in the workspace by additions that round.
+//
 // One sequence has few units and waits mostly for sums to travel: there the thread blocks come in clusters of eight, each
 // key head is cut into whole clusters of shares, and a cluster's sums meet in distributed shared memory; the workspace is
 // left for units that take several clusters.
@@ -160,6 +164,7 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
     constexpr uint32_t kRows = 8 * R;
     constexpr uint32_t kChunks = D / 8;          // 16-byte pieces of a row
     constexpr uint32_t kItem = Ring<D>::item, kItems = Ring<D>::items;
+    constexpr uint32_t kFold = std::is_same<T, __half>::value ? kFoldStepsF16 : kFoldStepsBF16;
     extern __shared__ __align__(128) uint8_t smem[];
     // [query rows][rings of the warps]; the rings' place is also where the warps' sums meet
     T *const query = reinterpret_cast<T *>(smem);
@@ -250,9 +255,12 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
     do {
         const uint32_t unit_count = u.groups.count();
         const uint64_t unit_end = unit_begin + unit_count;
-        const uint32_t g0 = (uint32_t)(position - unit_begin), g1 = (uint32_t)(min(unit_end, end) - unit_begin);
+        // A long range is taken in pieces, so that no warp's chain of products gets longer than the sums bear: all but the last
+        // leave theirs in the workspace.
+        const uint32_t g0 = (uint32_t)(position - unit_begin);
+        const uint32_t g1 = min((uint32_t)(min(unit_end, end) - unit_begin), g0 + kWarps * kFold);
+        const bool last_piece = unit_begin + g1 == min(unit_end, end);
         const uint32_t unit_row0 = u.chunk * kRows, unit_rows = min(kRows, u.rows.count * p.group - unit_row0);
-        const bool whole = g0 == 0 && g1 == unit_count;
         const int64_t place0 = (int64_t)u.rows.length - u.rows.count;  // of the sequence's first new token
         const uint32_t keys_end = u.groups.end == 0 ? 0 : u.rows.length;
         const uint32_t *table = p.batch.table + (size_t)u.sequence * p.batch.table_stride;
@@ -496,6 +504,43 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
             }
         }
         __syncthreads();
+        const bool whole = unit_begin >= begin && unit_end <= end;
+        const bool first_piece = position == max(begin, unit_begin);
+        // four outputs over the warps and the pieces in front of this one; false: they wait for the next piece
+        float *const folds = p.folds + (size_t)blockIdx.x * kFoldFloats;  // every thread reads what it wrote
+        auto gather = [&](uint32_t i, uint32_t row, uint32_t column, float4 &sum, float &high, float &mass) {
+            sum = make_float4(0, 0, 0, 0);
+            high = -INFINITY;
+            mass = 0.0f;
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) high = fmaxf(high, top_of[w][row]);
+#pragma unroll
+            for (uint32_t w = 0; w < kWarps; ++w) {
+                const float4 part = *reinterpret_cast<const float4 *>(sums + (w * kRows + row) * kSumRow + column);
+                sum.x += part.x; sum.y += part.y; sum.z += part.z; sum.w += part.w;
+                mass += top_of[w][row] == -INFINITY ? total_of[w][row] : total_of[w][row] * exp2_fast(top_of[w][row] - high);
+            }
+            if (first_piece && last_piece) return true;
+            float4 *const fold = reinterpret_cast<float4 *>(folds) + i;
+            float2 *const told = reinterpret_cast<float2 *>(folds + kMostRows * kMostHead) + i;  // (top, total)
+            if (!first_piece) {
+                const float4 before = *fold;
+                const float grown = fmaxf(high, told->x);
+                const float keep = told->x == -INFINITY ? 1.0f : exp2_fast(told->x - grown);  // sums of nothing are zeros, or NaN
+                const float scaled = high == -INFINITY ? 1.0f : exp2_fast(high - grown);
+                sum.x = sum.x * scaled + before.x * keep;
+                sum.y = sum.y * scaled + before.y * keep;
+                sum.z = sum.z * scaled + before.z * keep;
+                sum.w = sum.w * scaled + before.w * keep;
+                mass = mass * scaled + told->y * keep;
+                high = grown;
+            }
+            if (!last_piece) {
+                *fold = sum;
+                *told = make_float2(high, mass);
+            }
+            return last_piece;
+        };
         if (CLUSTER && unit_stride != 0) {
             cg::cluster_group cluster = cg::this_cluster();
             const uint32_t rank = cluster.block_rank(), items = unit_rows * (D / 4);
@@ -503,21 +548,18 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
                         *const own_total = own_top + kRows;
             for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
                 const uint32_t row = i / (D / 4), column = (i % (D / 4)) * 4;
-                float4 sum = make_float4(0, 0, 0, 0);
-                float high = -INFINITY, mass = 0.0f;
-#pragma unroll
-                for (uint32_t w = 0; w < kWarps; ++w) high = fmaxf(high, top_of[w][row]);
-#pragma unroll
-                for (uint32_t w = 0; w < kWarps; ++w) {
-                    const float4 part = *reinterpret_cast<const float4 *>(sums + (w * kRows + row) * kSumRow + column);
-                    sum.x += part.x; sum.y += part.y; sum.z += part.z; sum.w += part.w;
-                    mass += top_of[w][row] == -INFINITY ? total_of[w][row] : total_of[w][row] * exp2_fast(top_of[w][row] - high);
-                }
+                float4 sum;
+                float high, mass;
+                if (!gather(i, row, column, sum, high, mass)) continue;
                 *reinterpret_cast<float4 *>(own_sum + row * D + column) = sum;
                 if (column == 0) {
                     own_top[row] = high;
                     own_total[row] = mass;
                 }
+            }
+            if (!last_piece) {
+                position = unit_begin + g1;
+                continue;
             }
             cluster.sync();
             // every block adds an eighth of the outputs up over the cluster
@@ -619,16 +661,9 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
         float *const partial = p.partials + (size_t)slot * kSlotFloats;  // [rows][D], then maxima, then totals
         for (uint32_t i = threadIdx.x; i < unit_rows * (D / 4); i += kThreads) {
             const uint32_t row = i / (D / 4), column = (i % (D / 4)) * 4;
-            float4 sum = make_float4(0, 0, 0, 0);
-            float high = -INFINITY, mass = 0.0f;
-#pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) high = fmaxf(high, top_of[w][row]);
-#pragma unroll
-            for (uint32_t w = 0; w < kWarps; ++w) {
-                const float4 part = *reinterpret_cast<const float4 *>(sums + (w * kRows + row) * kSumRow + column);
-                sum.x += part.x; sum.y += part.y; sum.z += part.z; sum.w += part.w;
-                mass += top_of[w][row] == -INFINITY ? total_of[w][row] : total_of[w][row] * exp2_fast(top_of[w][row] - high);
-            }
+            float4 sum;
+            float high, mass;
+            if (!gather(i, row, column, sum, high, mass)) continue;
             if (whole) {
                 const uint32_t flat = unit_row0 + row;
                 T *to = static_cast<T *>(p.out) + (size_t)(u.rows.begin + flat / p.group) * p.ldo +
@@ -642,6 +677,10 @@ attend_kernel(const __grid_constant__ AttentionArgs p) {
                     partial[kMostRows * (kMostHead + 1) + row] = mass;
                 }
             }
+        }
+        if (!last_piece) {
+            position = unit_begin + g1;
+            continue;
         }
         if (!whole) {
             __threadfence();
@@ -790,7 +829,9 @@ cudaError_t launch_head(const AttentionArgs &args, int sm_count, cudaStream_t st
 size_t attention_partial_bytes(int sm_count) {
     return (size_t)sm_count * kBlocksPerSm * 2 * kMostRows * (kMostHead + 2) * sizeof(float);
 }
-size_t attention_arrival_bytes(int sm_count) { return (size_t)sm_count * kBlocksPerSm * sizeof(uint32_t); }
+size_t attention_fold_bytes(int sm_count) { return (size_t)sm_count * kBlocksPerSm * kFoldFloats * sizeof(float); }
+// a counter per thread block, and behind them the owners of the folded sums (a prompt's thread blocks are more than SMs)
+size_t attention_arrival_bytes(int sm_count) { return (size_t)sm_count * kBlocksPerSm * 2 * sizeof(uint32_t); }
 
 cudaError_t launch_attention(const AttentionArgs &args, int sm_count, cudaStream_t stream) {
     const uint64_t rows = (uint64_t)(args.most_tokens != 0 ? args.most_tokens : args.batch.tokens) * args.group;

@@ -164,11 +164,19 @@ struct AttentionArgs {
     float scale;
     uint32_t window, sinks;
     float *partials;       // attention_partial_bytes of scratch
+    float *folds;          // behind them: kFoldFloats for every SM
     uint32_t *arrivals;    // attention_arrival_bytes, zero between launches
     uint32_t *status;
 };
-// what every attention launch of a device may use: sums of split rows and their counters
+// Matrix instructions cut a running sum off instead of rounding it: after n of them it is up to n 2^-23 of itself too small
+// (measured: 2^-23 for each).  Behind this many a thread block's sums are folded into others in scratch of its own, by
+// additions that round, so that what is lost stays below a quarter of the half step that the output's rounding may be off
+// by (2^-12 of a value in fp16, 2^-9 in bf16).
+constexpr uint32_t kFoldStepsF16 = 512, kFoldStepsBF16 = 4096;
+constexpr size_t kFoldFloats = 128 * 256;
+// what every attention launch of a device may use: sums of split rows and their counters, folded sums
 size_t attention_partial_bytes(int sm_count);
+size_t attention_fold_bytes(int sm_count);
 size_t attention_arrival_bytes(int sm_count);
 cudaError_t launch_attention(const AttentionArgs &args, int sm_count, cudaStream_t stream);
 // ---- q4b_prompt.cu: the same for many rows per sequence, on tcgen05 ----

@@ -29,6 +29,11 @@
 // row sees becomes zero, and an infinity or a NaN that some rows see and others do not (0 x infinity is NaN) sends the
 // unit through a plain fp32 loop at the end.
 //
+// The tensor cores cut a running sum off where they would have to round it: after the 65,536 products of a million keys O
+// was too small by 0.7%.  So every 64 tiles (fp16; 512 in bf16) the softmax's warps fold O into fp32 sums in the workspace,
+// by additions that round, and O starts again; at the end what was folded comes back.  The place for that, 128 KB, is lent to
+// the thread block.  The loop over tiles is in two levels for it: with the fold inside, tiles took 2 to 6% longer.
+//
 // When there are fewer units than SMs the keys of a unit are split over a cluster of 2 to 8 thread blocks, whose sums meet
 // in distributed shared memory.
 //
@@ -70,7 +75,24 @@ struct PromptParams {
     CUtensorMap k_map, v_map;   // [D / 64][pages x kv_heads x page_tokens][64]
     AttentionArgs a;
     uint32_t units, splits, k_shift, v_shift;  // boxes of 1 << k_shift, 1 << v_shift tokens
+    uint32_t sms;
 };
+
+// A place for folded sums: one per SM, and a thread block that needs one has an SM to itself, so one of them is free --
+// most likely that of this SM's number.  kNoPlace when none is, which the host hears of.
+constexpr uint32_t kNoPlace = 0xffffffffu;
+__device__ inline uint32_t take_place(uint32_t *owners, uint32_t places) {
+    uint32_t sm;
+    asm volatile("mov.u32 %0, %%smid;" : "=r"(sm));
+    for (uint32_t i = 0; i < 4 * places; ++i) {
+        const uint32_t at = (sm + i) % places;
+        if (atomicCAS(owners + at, 0u, 1u) == 0) {
+            __threadfence();
+            return at;
+        }
+    }
+    return kNoPlace;
+}
 
 __device__ inline float exp2_of(float x) {
     float y;
@@ -162,6 +184,28 @@ struct Unit {
     }
 };
 
+// A row's sums in TMEM and, times the factor, what was folded of them before (nothing the first time): into the folded ones,
+// or back into TMEM.  Not inlined: it is rare.
+__device__ __noinline__ void fold_columns(uint32_t columns, uint32_t count, float *folded, float factor, bool first, bool back) {
+#pragma unroll 1
+    for (uint32_t column = 0; column < count; column += 32) {
+        uint32_t o[32];
+        float *const at = folded + (size_t)column * kTileRowsQ;
+        tc_load_32(columns + column, o);
+        tc_wait_loaded(o);
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (!first) o[i] = __float_as_uint(fmaf(__ldcg(at + i * kTileRowsQ), factor, __uint_as_float(o[i])));
+        if (back) {
+            tc_store_32(columns + column, o);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) __stcg(at + i * kTileRowsQ, __uint_as_float(o[i]));
+        }
+    }
+    if (back) tc_wait_store();
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(kPromptThreads, 1)
 prompt_kernel(const __grid_constant__ PromptParams p) {
@@ -172,7 +216,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     uint8_t *const misc = ring + 2 * S::slots * kSlotBytes;
     float *const exchange = reinterpret_cast<float *>(misc);                    // [2][128]
     uint64_t *const bars = reinterpret_cast<uint64_t *>(misc + 1024);
-    uint32_t *const words = reinterpret_cast<uint32_t *>(bars + 4 * S::slots + 8);  // TMEM address, poison flag
+    uint32_t *const words = reinterpret_cast<uint32_t *>(bars + 4 * S::slots + 8);  // TMEM address, poison flag, place of folds
     const uint32_t k_full0 = tc_smem_u32(bars), k_empty0 = k_full0 + 8 * S::slots, v_full0 = k_empty0 + 8 * S::slots,
                    v_empty0 = v_full0 + 8 * S::slots;
     const uint32_t k_ring = tc_smem_u32(ring), v_ring = k_ring + S::slots * kSlotBytes;
@@ -223,6 +267,8 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
         u.size = (uint32_t)((uint64_t)all * (rank + 1) / p.splits) - u.first;
     }
     const uint32_t n = u.size;
+    constexpr uint32_t kFold = (std::is_same<T, __half>::value ? kFoldStepsF16 : kFoldStepsBF16) * 16 / kTileKeys;  // tiles
+    const bool folds = n > kFold;
     const uint32_t *const table = a.batch.table + (size_t)u.sequence * a.batch.table_stride;
 
     if (threadIdx.x == 0) {
@@ -236,6 +282,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
         tc_mbar_init(v_look, 1);
         tc_mbar_init(v_ready, 32);
         words[1] = 0;
+        words[2] = folds ? take_place(a.arrivals + p.sms, p.sms) : 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -248,7 +295,8 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = words[0], tmem_o = tmem, tmem_s = tmem + 256;
-    bool ok = true;
+    const uint32_t place_of_folds = words[2];
+    bool ok = place_of_folds != kNoPlace;
 
     if (warp == 0 || warp == 2) {
         // ---- producers: warp 0 the keys, warp 2 the values ----
@@ -353,13 +401,14 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 tc_commit_by(leader, s_full0 + 8 * (j & 1));
                 return true;
             };
-            ok = tc_warp_wait(q_full, 0);
+            ok = ok && tc_warp_wait(q_full, 0);
             tc_fence_after();
             if (ok) ok = scores(0);
             if (ok && n > 1) ok = scores(1);
             for (uint32_t j = 0; j < n && ok; ++j) {
                 // the values came long ago: their waits (100 clocks each) are over before the weights are there
                 uint32_t slot = v_slot, lap = v_lap;
+                if (j % kFold == 0) begun = 0;  // what O holds has been folded before these weights were handed over
 #pragma unroll
                 for (uint32_t part = 0; part < S::parts; ++part) {
                     if (ok) ok = tc_warp_wait(v_full0 + 8 * slot, lap & 1);
@@ -506,86 +555,106 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             const bool active = quad * 32 < u.count;  // otherwise none of the warp's rows is asked for
             const int64_t place = row < u.count ? u.place0 + (u.row0 + row) / a.group : -1;
             float top = -INFINITY, total = 0.0f;
-            for (uint32_t j = 0; j < n; ++j) {
-                // found out while S(j) is on its way: are there columns to hide, and which
-                const uint32_t key0 = u.key(j);
-                const bool edge = !u.clear(a, key0);
-                if (ok && !tc_wait(s_full0 + 8 * (j & 1), (j >> 1) & 1)) ok = false;
+            float folded_top = -INFINITY, folded_total = 0.0f;
+            // [columns][128 rows]: every thread reads what it wrote
+            float *const folded = a.folds + (size_t)place_of_folds * kFoldFloats + (size_t)half * (D / 2) * kTileRowsQ + row;
+            auto fold = [&](uint32_t next, bool back) {  // O holds the sums of the tiles before `next`
+                if (ok && !tc_wait(o_done, (next - 1) & 1)) ok = false;
+                if (!ok || !active) return;
+                const float factor = folded_top == -INFINITY ? 0.0f : exp2_of(folded_top - top);
                 tc_fence_after();
-                const uint32_t s_columns = tmem_s + (j & 1) * 128 + lanes;
-                if (active) {
-                    uint32_t raw[2][32];
-                    tc_load_32(s_columns + half * 64, raw[0]);
-                    tc_load_32(s_columns + half * 64 + 32, raw[1]);
-                    tc_wait_loaded(raw[0]);
-                    tc_wait_loaded(raw[1]);
-                    if (edge) {
-                        // visible columns: below `behind`, and from `from` on or below `sink`
-                        const int64_t first = (int64_t)key0 + half * 64;
-                        const int32_t behind = (int32_t)max((int64_t)0, min((int64_t)64, place + 1 - first));
-                        const int32_t from = a.window == 0 ? 0 : (int32_t)max((int64_t)0, min((int64_t)64, place - (int64_t)a.window + 1 - first));
-                        const int32_t sink = (int32_t)max((int64_t)0, min((int64_t)64, (int64_t)a.sinks - first));
+                fold_columns(tmem_o + lanes + half * (D / 2), D / 2, folded, factor, next == kFold, back);
+                folded_total = fmaf(folded_total, factor, total);
+                folded_top = top;
+                total = 0.0f;
+            };
+            for (uint32_t j0 = 0; j0 < n; j0 += kFold) {
+                if (j0 != 0) fold(j0, false);
+                for (uint32_t j = j0; j < min(n, j0 + kFold); ++j) {
+                    // found out while S(j) is on its way: are there columns to hide, and which
+                    const uint32_t key0 = u.key(j);
+                    const bool edge = !u.clear(a, key0);
+                    if (ok && !tc_wait(s_full0 + 8 * (j & 1), (j >> 1) & 1)) ok = false;
+                    tc_fence_after();
+                    const uint32_t s_columns = tmem_s + (j & 1) * 128 + lanes;
+                    if (active) {
+                        uint32_t raw[2][32];
+                        tc_load_32(s_columns + half * 64, raw[0]);
+                        tc_load_32(s_columns + half * 64 + 32, raw[1]);
+                        tc_wait_loaded(raw[0]);
+                        tc_wait_loaded(raw[1]);
+                        if (edge) {
+                            // visible columns: below `behind`, and from `from` on or below `sink`
+                            const int64_t first = (int64_t)key0 + half * 64;
+                            const int32_t behind = (int32_t)max((int64_t)0, min((int64_t)64, place + 1 - first));
+                            const int32_t from = a.window == 0 ? 0 : (int32_t)max((int64_t)0, min((int64_t)64, place - (int64_t)a.window + 1 - first));
+                            const int32_t sink = (int32_t)max((int64_t)0, min((int64_t)64, (int64_t)a.sinks - first));
 #pragma unroll
-                        for (int i = 0; i < 64; ++i) {
-                            if (!(i < behind && (i >= from || i < sink))) raw[i >> 5][i & 31] = 0xff800000u;  // -infinity
-                        }
-                    }
-                    float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int i = 0; i < 64; i += 2)
-                        most[i >> 1 & 3] = max3(most[i >> 1 & 3], __uint_as_float(raw[i >> 5][i & 31]), __uint_as_float(raw[i >> 5][i + 1 & 31]));
-                    float high = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
-                    pair_barrier(5 + quad);  // the other half has read what it was told last time
-                    exchange[half * 128 + row] = high;
-                    pair_barrier(1 + quad);
-                    high = fmaxf(high, exchange[(half ^ 1) * 128 + row]) * c - kLift<T>;
-                    const bool grow = high > top + kRescaleAt || (top == -INFINITY && high > -INFINITY);
-                    bool waited = j == 0;
-                    if (__any_sync(0xffffffffu, grow)) {
-                        const float factor = grow ? exp2_of(top - high) : 1.0f;
-                        if (grow) top = high;
-                        total *= factor;
-                        if (j > 0) {
-                            if (ok && !tc_wait(o_done, (j - 1) & 1)) ok = false;
-                            waited = true;
-                            tc_fence_after();
-#pragma unroll 1
-                            for (uint32_t column = half * (D / 2); column < (half + 1) * (D / 2); column += 32) {
-                                uint32_t o[32];
-                                tc_load_32(tmem_o + lanes + column, o);
-                                tc_wait_loaded(o);
-#pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
-                                tc_store_32(tmem_o + lanes + column, o);
+                            for (int i = 0; i < 64; ++i) {
+                                if (!(i < behind && (i >= from || i < sink))) raw[i >> 5][i & 31] = 0xff800000u;  // -infinity
                             }
                         }
-                    }
-                    const float minus = top == -INFINITY ? 0.0f : -top;
-                    uint32_t weights[32];
-                    const uint64_t factors = two(c, c), offsets = two(minus, minus);
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        float most[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const float2 x = apart(fma2(two(__uint_as_float(raw[i >> 4][(2 * i) & 31]), __uint_as_float(raw[i >> 4][(2 * i + 1) & 31])),
-                                              factors, offsets));
-                        weights[i] = pack2<T>(exp2_of(x.x), exp2_of(x.y));
-                        plus_weights<T>(sum[2 * (i & 1)], sum[2 * (i & 1) + 1], weights[i]);
+                        for (int i = 0; i < 64; i += 2)
+                            most[i >> 1 & 3] = max3(most[i >> 1 & 3], __uint_as_float(raw[i >> 5][i & 31]), __uint_as_float(raw[i >> 5][i + 1 & 31]));
+                        float high = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+                        pair_barrier(5 + quad);  // the other half has read what it was told last time
+                        exchange[half * 128 + row] = high;
+                        pair_barrier(1 + quad);
+                        high = fmaxf(high, exchange[(half ^ 1) * 128 + row]) * c - kLift<T>;
+                        const bool grow = high > top + kRescaleAt || (top == -INFINITY && high > -INFINITY);
+                        bool waited = j == 0;
+                        if (__any_sync(0xffffffffu, grow)) {
+                            const float factor = grow ? exp2_of(top - high) : 1.0f;
+                            if (grow) top = high;
+                            total *= factor;
+                            if (j > 0) {
+                                if (ok && !tc_wait(o_done, (j - 1) & 1)) ok = false;
+                                waited = true;
+                                tc_fence_after();
+#pragma unroll 1
+                                for (uint32_t column = half * (D / 2); column < (half + 1) * (D / 2); column += 32) {
+                                    uint32_t o[32];
+                                    tc_load_32(tmem_o + lanes + column, o);
+                                    tc_wait_loaded(o);
+#pragma unroll
+                                    for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * factor);
+                                    tc_store_32(tmem_o + lanes + column, o);
+                                }
+                            }
+                        }
+                        const float minus = top == -INFINITY ? 0.0f : -top;
+                        uint32_t weights[32];
+                        const uint64_t factors = two(c, c), offsets = two(minus, minus);
+                        float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const float2 x = apart(fma2(two(__uint_as_float(raw[i >> 4][(2 * i) & 31]), __uint_as_float(raw[i >> 4][(2 * i + 1) & 31])),
+                                                  factors, offsets));
+                            weights[i] = pack2<T>(exp2_of(x.x), exp2_of(x.y));
+                            plus_weights<T>(sum[2 * (i & 1)], sum[2 * (i & 1) + 1], weights[i]);
+                        }
+                        tc_store_32(s_columns + half * 32, weights);
+                        tc_wait_store();
+                        // O(j - 1) is complete long before P(j) is needed; every warp sees every round of its barrier
+                        if (!waited && ok && !tc_wait(o_done, (j - 1) & 1)) ok = false;
+                        total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    } else if (j > 0 && ok && !tc_wait(o_done, (j - 1) & 1)) {
+                        ok = false;
                     }
-                    total += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tc_store_32(s_columns + half * 32, weights);
-                    tc_wait_store();
-                    // O(j - 1) is complete long before P(j) is needed; every warp sees every round of its barrier
-                    if (!waited && ok && !tc_wait(o_done, (j - 1) & 1)) ok = false;
-                } else if (j > 0 && ok && !tc_wait(o_done, (j - 1) & 1)) {
-                    ok = false;
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) tc_mbar_arrive(p_full0 + 8 * (j & 1));
                 }
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) tc_mbar_arrive(p_full0 + 8 * (j & 1));
             }
             if (n > 0 && ok && !tc_wait(o_done, (n - 1) & 1)) ok = false;
             if (!ok && lane == 0) atomicExch(a.status, 0x84u);
             tc_fence_after();
+            if (folds) {  // what was folded comes back into O
+                fold(n, true);
+                total = folded_total;
+            }
             if (active) {
                 pair_barrier(5 + quad);
                 exchange[half * 128 + row] = total;
@@ -661,6 +730,10 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (threadIdx.x == 0 && folds && place_of_folds != kNoPlace) {
+        __threadfence();
+        atomicExch(a.arrivals + p.sms + place_of_folds, 0u);
+    }
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
     }
@@ -680,6 +753,9 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 sum[i] = 0.0f;
             }
             for (uint32_t j = 0; j < n; ++j) {
+                float tile_sum[D / 32], tile_top = -INFINITY, tile_total = 0.0f;  // no long chain of additions
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) tile_sum[i] = 0.0f;
                 for (uint32_t key = u.key(j); key < u.key(j) + kTileKeys; ++key) {
                     if ((int64_t)key > place || !(a.window == 0 || (int64_t)key > place - (int64_t)a.window || key < a.sinks)) continue;
                     const uint32_t page = __ldg(table + (key >> a.cache.page_shift));
@@ -691,15 +767,23 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     for (int i = 0; i < D / 32; ++i) score += mine[i] * wide(static_cast<const T *>(a.cache.keys)[line + i * 32 + lane]);
 #pragma unroll
                     for (int d = 16; d > 0; d >>= 1) score += __shfl_xor_sync(0xffffffffu, score, d);
-                    const float high = fmaxf(top, score);
+                    const float high = fmaxf(tile_top, score);
                     const float minus = high == -INFINITY ? 0.0f : high;
-                    const float keep = exp2_of(top - minus), weight = exp2_of(score - minus);
-                    top = high;
-                    total = total * keep + weight;
+                    const float keep = exp2_of(tile_top - minus), weight = exp2_of(score - minus);
+                    tile_top = high;
+                    tile_total = tile_total * keep + weight;
 #pragma unroll
                     for (int i = 0; i < D / 32; ++i)
-                        sum[i] = sum[i] * keep + weight * wide(static_cast<const T *>(a.cache.values)[line + i * 32 + lane]);
+                        tile_sum[i] = tile_sum[i] * keep + weight * wide(static_cast<const T *>(a.cache.values)[line + i * 32 + lane]);
                 }
+                const float high = fmaxf(top, tile_top);
+                const float minus = high == -INFINITY ? 0.0f : high;
+                // what saw nothing has sums of zero (or NaN)
+                const float keep = top == -INFINITY ? 1.0f : exp2_of(top - minus), scale = tile_top == -INFINITY ? 1.0f : exp2_of(tile_top - minus);
+                top = high;
+                total = total * keep + tile_total * scale;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) sum[i] = sum[i] * keep + tile_sum[i] * scale;
             }
             if (p.splits == 1) {
                 T *const to = static_cast<T *>(a.out) + (size_t)(u.rows.begin + flat / a.group) * a.ldo +
@@ -832,6 +916,7 @@ cudaError_t launch_prompt_of(const AttentionArgs &args, int sm_count, cudaStream
         if (units <= (uint64_t)here[k]) p.splits = k;
     if (units * p.splits > 0x7fffffffu) return cudaErrorInvalidConfiguration;
     p.units = (uint32_t)units;
+    p.sms = (uint32_t)sm_count;
     config.gridDim = dim3((unsigned)(units * p.splits));
     attribute[0].val.clusterDim.x = p.splits;
     return cudaLaunchKernelEx(&config, prompt_kernel<T, D>, p);
