@@ -494,10 +494,13 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             // row sees them, no infinity where only some do ----
             constexpr uint32_t exponent = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
             constexpr uint32_t both = exponent | exponent << 16, low = std::is_same<T, __half>::value ? 0x04000400u : 0x00800080u;
-            uint32_t looked = 0;
+            uint32_t looked = 0, passed = 0;
             for (uint32_t j = 0; j < n && ok; ++j) {
                 const uint32_t key0 = u.key(j);
-                if (u.clear(a, key0)) continue;
+                if (u.clear(a, key0)) {
+                    ++passed;
+                    continue;
+                }
                 // a bit per key: nobody sees it, some do and some do not; four words of 32 keys
                 uint32_t nobody[4], some[4];
 #pragma unroll
@@ -506,8 +509,13 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     nobody[w] = __ballot_sync(0xffffffffu, !any);
                     some[w] = __ballot_sync(0xffffffffu, any && !every);
                 }
-                ok = tc_warp_wait(v_look, looked & 1);
+                // the tiles in between may take longer than one wait bears: 2^15 tiles of up to 120,000 clocks for each
+                for (uint32_t patience = passed >> 15;; --patience) {
+                    ok = tc_warp_wait(v_look, looked & 1);
+                    if (ok || patience == 0) break;
+                }
                 if (!ok) break;
+                passed = 0;
                 ++looked;
                 uint32_t strange = 0;
 #pragma unroll

@@ -124,3 +124,10 @@ def test_an_infinity_at_the_end_of_a_long_context(q4b, ctx, dtype, most_tokens):
     assert (got[:-1] == want).all()
     assert not np.isfinite(widen(got[-1][:, ::3], dtype)).any()
     assert (got[-1] == want)[:, np.arange(64) % 3 != 0].all()
+
+
+def test_a_context_that_takes_longer_than_one_wait(q4b, ctx):
+    """268 million tokens: between a unit's first and its masked last tile pass more clocks than a bounded wait lasts, and the
+    warp that looks at the last tile's values waits all that time."""
+    case = Long(q4b, ctx, "bf16", 64, 3, 16, 1, 280, 2 ** 28 + 17, equal=True)
+    case.check_equal(case.run(280))
