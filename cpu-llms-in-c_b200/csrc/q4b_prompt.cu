@@ -576,9 +576,8 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 folded_top = top;
                 total = 0.0f;
             };
-            for (uint32_t j0 = 0; j0 < n; j0 += kFold) {
-                if (j0 != 0) fold(j0, false);
-                for (uint32_t j = j0; j < min(n, j0 + kFold); ++j) {
+            for (uint32_t j = 0, stop = min(n, kFold);;) {
+                for (; j < stop; ++j) {
                     // found out while S(j) is on its way: are there columns to hide, and which
                     const uint32_t key0 = u.key(j);
                     const bool edge = !u.clear(a, key0);
@@ -655,6 +654,9 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                     __syncwarp();
                     if (lane == 0) tc_mbar_arrive(p_full0 + 8 * (j & 1));
                 }
+                if (j == n) break;
+                fold(j, false);
+                stop = min(n, j + kFold);
             }
             if (n > 0 && ok && !tc_wait(o_done, (n - 1) & 1)) ok = false;
             if (!ok && lane == 0) atomicExch(a.status, 0x84u);
