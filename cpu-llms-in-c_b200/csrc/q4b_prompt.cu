@@ -18,7 +18,7 @@
 // Weights meet the values in 16 bits, as the tensor cores take them, and a row's sum takes them so too: what the rounding
 // does to a weight it then does to numerator and denominator alike, and equal values come back as they are.  Summed as they
 // were before it, a row that one key dominates is off by a rounding more: behind the first tile that key's weight is any
-// number.  The sum by the mixed addition costs 0.6% of 8,192 tokens' time (1.6% with the weights widened first), 2% of a
+// number.  The sum by the mixed addition cost 0.6% of 8,192 tokens' time (1.6% with the weights widened first), 2% of a
 // verify step's.  A second product with what the rounding leaves out would bring the error down from 1.2 to 1.4 times that
 // of fp32 weights, for 1,024 more of a tile's 2,048 clocks of products.
 //
@@ -40,9 +40,9 @@
 // What bounds it: keys and values from L2, 512 D bytes per tile and SM.  At D = 256 the ring holds 1.25 tiles and 42 bytes
 // per clock and SM arrive (more than 10 TB/s over the chip); a tile takes some 3,000 clocks, 2,048 of them products.
 // Measured on B200 (fp16 and bf16 alike), in bursts of 20 calls: a prompt of 8,192 tokens, 24 query heads on 4 key heads of
-// 256, 748 us = 1,103 TFLOP/s of 1,677; four prompts of up to 4,001 tokens behind a window of 1,024, 446 us; 511 tokens behind
-// 30,001, 16 heads on 4 of 128, 156 us = 810 TFLOP/s; four tokens of six users behind a window of 4,096, 32 us.  Called for
-// seconds, under the power cap, the first takes 853 us and the third 165.
+// 256, 751 us = 1,098 TFLOP/s of 1,677; four prompts of up to 4,001 tokens behind a window of 1,024, 438 us; 511 tokens behind
+// 30,001, 16 heads on 4 of 128, 162 us = 782 TFLOP/s; four tokens of six users behind a window of 4,096, 32 us.  Called for
+// seconds, under the power cap, the first takes 858 us and the third 169.
 #include "q4b_cache.cuh"
 #include "q4b_tc.cuh"
 
