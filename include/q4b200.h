@@ -312,7 +312,7 @@ int q4b_rope_append(q4b_context *context, const q4b_kv_cache *cache, const q4b_t
  * zeros.  What is not visible has no influence, whatever it holds, infinities and NaN included; in calls of many rows
  * per sequence a value of that kind which some rows see and others do not has its keys gone through one by one: right,
  * but orders of magnitude slower.  The result does not depend on timing.  The first call on a context allocates a
- * workspace (never while recording).  Asynchronous. */
+ * workspace (24 MB on a B200; never while recording).  Asynchronous. */
 int q4b_attention(q4b_context *context, const q4b_kv_cache *cache, const q4b_token_batch *batch, const void *q,
                   uint32_t ldq, uint32_t q_heads, float scale, uint32_t window, uint32_t sinks, void *out, uint32_t ldo,
                   char *error_message, size_t error_capacity);

@@ -131,3 +131,50 @@ def test_a_context_that_takes_longer_than_one_wait(q4b, ctx):
     warp that looks at the last tile's values waits all that time."""
     case = Long(q4b, ctx, "bf16", 64, 3, 16, 1, 280, 2 ** 28 + 17, equal=True)
     case.check_equal(case.run(280))
+
+
+def test_two_contexts_fold_at_once(q4b):
+    """Each lends places of its own; their thread blocks share the chip."""
+    import threading
+    failures = []
+
+    def work(seed):
+        try:
+            with q4b.Q4Context(0) as own:
+                for shape in ((3, 16, 1, 280, 2 ** 17 + 17), (1, 6, 1, 40, 2 ** 20 + 5), (2, 4, 150, 1, 2 ** 20 + 17)):
+                    case = Long(q4b, own, "f16", 64, *shape, equal=True, seed=seed)
+                    for _ in range(3):
+                        case.check_equal(case.run(shape[3]))
+        except BaseException as error:  # noqa: BLE001 -- told to the test
+            failures.append(error)
+    threads = [threading.Thread(target=work, args=(seed,)) for seed in (31, 32)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not failures, failures
+
+
+def test_recorded_calls_that_fold(q4b, ctx):
+    """Two graphs share the workspace and its places; the lengths move between replays, across and back behind a fold."""
+    runs = []
+    for shape in ((3, 16, 1, 280, 40_000), (1, 16, 150, 1, 2 ** 17)):
+        case = Long(q4b, ctx, "f16", 64, *shape, equal=True)
+        case.run(shape[3])
+        held = [ctx.to_device(x) for x in (case.keys, case.values, case.table, case.q, np.full(case.sequences, case.length, np.uint32),
+                                           np.arange(case.sequences + 1, dtype=np.uint32) * case.new)]
+        out = ctx.alloc(case.q.nbytes)
+        cache = q4b.KVCache(keys=held[0].ptr, values=held[1].ptr, dtype=q4b.F16, pages=PAGES, page_tokens=PAGE,
+                            kv_heads=case.kv_heads, head_size=64)
+        batch = q4b.TokenBatch(sequences=case.sequences, tokens=len(case.q), most_tokens=case.new, token_begin=held[5].ptr,
+                               lengths=held[4].ptr, page_table=held[2].ptr, table_stride=case.columns)
+        ctx.graph_begin()
+        ctx.attention(cache, batch, held[3].ptr, case.kv_heads * case.group, out.ptr, case.scale)
+        runs.append((case, held, out, ctx.graph_end()))
+    for length in (40_000, 5_000, 8_193, 300, 39_999):
+        for case, held, out, graph in runs:
+            held[4].upload(np.full(case.sequences, length * (case.length // 40_000), np.uint32))
+            graph.launch()
+            graph.launch()
+            case.check_equal(out.download(np.float16, case.q.shape))
+    ctx.sync()
