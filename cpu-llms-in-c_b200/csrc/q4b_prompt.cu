@@ -40,7 +40,7 @@
 // What bounds it: keys and values from L2, 512 D bytes per tile and SM.  At D = 256 the ring holds 1.25 tiles and 42 bytes
 // per clock and SM arrive (more than 10 TB/s over the chip); a tile takes some 3,000 clocks, 2,048 of them products.
 // Measured on B200 (fp16 and bf16 alike), in bursts of 20 calls: a prompt of 8,192 tokens, 24 query heads on 4 key heads of
-// 256, 751 us = 1,098 TFLOP/s of 1,677; four prompts of up to 4,001 tokens behind a window of 1,024, 438 us; 511 tokens behind
+// 256, 751 us = 1,098 TFLOP/s of 1,677; four prompts of up to 4,001 tokens behind a window of 1,024, 434 us; 511 tokens behind
 // 30,001, 16 heads on 4 of 128, 162 us = 782 TFLOP/s; four tokens of six users behind a window of 4,096, 32 us.  Called for
 // seconds, under the power cap, the first takes 858 us and the third 169.
 #include "q4b_cache.cuh"
@@ -79,7 +79,7 @@ struct PromptParams {
 };
 
 // A place for folded sums: one per SM, and a thread block that needs one has an SM to itself, so one of them is free --
-// most likely that of this SM's number.  kNoPlace when none is, which the host hears of.
+// most likely that of this SM's number.  kNoPlace when none is.
 constexpr uint32_t kNoPlace = 0xffffffffu;
 __device__ inline uint32_t take_place(uint32_t *owners, uint32_t places) {
     uint32_t sm;
@@ -271,6 +271,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     const bool folds = n > kFold;
     const uint32_t *const table = a.batch.table + (size_t)u.sequence * a.batch.table_stride;
 
+    uint32_t own_place = kNoPlace;  // the first thread's to give back
     if (threadIdx.x == 0) {
         for (uint32_t s = 0; s < 4 * S::slots; ++s) tc_mbar_init(k_full0 + 8 * s, 1);  // full and empty of both rings
         tc_mbar_init(q_full, kPromptThreads - 96);
@@ -282,7 +283,11 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
         tc_mbar_init(v_look, 1);
         tc_mbar_init(v_ready, 32);
         words[1] = 0;
-        words[2] = folds ? take_place(a.arrivals + p.sms, p.sms) : 0;
+        if (folds) {
+            own_place = take_place(a.arrivals + p.sms, p.sms);
+            if (own_place == kNoPlace) atomicExch(a.status, 0x86u);  // cannot be; the results are then not to be used
+            words[2] = own_place == kNoPlace ? 0 : own_place;
+        }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -295,8 +300,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = words[0], tmem_o = tmem, tmem_s = tmem + 256;
-    const uint32_t place_of_folds = words[2];
-    bool ok = place_of_folds != kNoPlace;
+    bool ok = true;
 
     if (warp == 0 || warp == 2) {
         // ---- producers: warp 0 the keys, warp 2 the values ----
@@ -401,7 +405,7 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
                 tc_commit_by(leader, s_full0 + 8 * (j & 1));
                 return true;
             };
-            ok = ok && tc_warp_wait(q_full, 0);
+            ok = tc_warp_wait(q_full, 0);
             tc_fence_after();
             if (ok) ok = scores(0);
             if (ok && n > 1) ok = scores(1);
@@ -564,11 +568,11 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
             const int64_t place = row < u.count ? u.place0 + (u.row0 + row) / a.group : -1;
             float top = -INFINITY, total = 0.0f;
             float folded_top = -INFINITY, folded_total = 0.0f;
-            // [columns][128 rows]: every thread reads what it wrote
-            float *const folded = a.folds + (size_t)place_of_folds * kFoldFloats + (size_t)half * (D / 2) * kTileRowsQ + row;
             auto fold = [&](uint32_t next, bool back) {  // O holds the sums of the tiles before `next`
                 if (ok && !tc_wait(o_done, (next - 1) & 1)) ok = false;
                 if (!ok || !active) return;
+                // [columns][128 rows]: every thread reads what it wrote
+                float *const folded = a.folds + (size_t)words[2] * kFoldFloats + (size_t)half * (D / 2) * kTileRowsQ + row;
                 const float factor = folded_top == -INFINITY ? 0.0f : exp2_of(folded_top - top);
                 tc_fence_after();
                 fold_columns(tmem_o + lanes + half * (D / 2), D / 2, folded, factor, next == kFold, back);
@@ -740,9 +744,9 @@ prompt_kernel(const __grid_constant__ PromptParams p) {
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (threadIdx.x == 0 && folds && place_of_folds != kNoPlace) {
+    if (own_place != kNoPlace) {
         __threadfence();
-        atomicExch(a.arrivals + p.sms + place_of_folds, 0u);
+        atomicExch(a.arrivals + p.sms + own_place, 0u);
     }
     if (warp == 1) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u));
